@@ -11,6 +11,15 @@ from .frontend import (
     compile,
     compile_training,
 )
+from .losses import (
+    policy_loss,
+    policy_loss_and_grad,
+    preference_loss,
+    preference_loss_and_grad,
+    token_logprobs,
+    token_logprobs_and_grad,
+)
+from .optim import AdamW, AdamWState
 
 __version__ = "0.1.0"
 
@@ -24,4 +33,12 @@ __all__ = [
     "capture",
     "compile",
     "compile_training",
+    "token_logprobs",
+    "token_logprobs_and_grad",
+    "policy_loss",
+    "policy_loss_and_grad",
+    "preference_loss",
+    "preference_loss_and_grad",
+    "AdamW",
+    "AdamWState",
 ]

@@ -1,0 +1,332 @@
+// AdamW over many tensors in one launch, moments in 32 or in 8 bits.
+//
+// Mathematics, per element, with t steps taken including this one:
+//     m' = b1 m + (1 - b1) g,   v' = b2 v + (1 - b2) g^2,
+//     p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps).
+// In 8 bits a block of 256 elements shares one FP32 scale per moment, m is held as e4m3 times its scale, and of v the
+// square root, which needs half the exponent range.  Rounding to nearest would stop both moments: with b2 = 0.999 a root
+// moves by at most 0.05 % a step towards zero, and the nearest e4m3 number is up to 6 % away, so the code would never
+// change.  Both are rounded up with the probability of the part that is cut (the expected value is the unrounded one); the
+// 16 random bits come from a hash of the element's place and the step, so a run repeats exactly.  A root above zero is
+// never rounded to zero, which would divide by eps alone.  The update itself uses the unrounded moments.  The products and
+// sums of the moments, their scales and the scaled values are rounded one by one (no fused multiply-add): which way a value
+// on a border is rounded then follows from the formulas alone, in whatever form they are compiled.
+#include "tk_ops_host.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cmath>
+
+namespace {
+
+using tk_ops::check;
+using tk_ops::count_launch;
+using tk_ops::DeviceScope;
+using tk_ops::fail;
+
+constexpr int kThreads = 256;
+constexpr int kPerThread = 8;
+constexpr int kChunk = kThreads * kPerThread;     // elements one block updates at a time: 8 scale blocks, one per warp
+constexpr int kFew = 64, kMany = 768;             // tensors in one launch's parameter block (at most 32,764 bytes)
+constexpr float kE4m3Max = 448.f;
+constexpr float kSmallest = 7.888609052e-31f;      // 2^-100: a block whose largest value is below it is held as zeros (448 / value stays finite)
+
+struct Item {
+    void* param;
+    const void* grad;
+    int64_t offset, count;
+    int32_t first_chunk;
+    float weight_decay;
+};
+
+template <int CAPACITY>
+struct Args {
+    tk_adamw_state state;
+    const float *lr_at, *scale_at;
+    double log_beta1, log_beta2;
+    float lr, beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
+    uint32_t seed;
+    int32_t count, chunks, last;
+    Item items[CAPACITY];
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// A 32-bit mixing function of two multiplications (xor-shift-multiply, constants from C. Wellons' published search for
+// low-bias hashes, https://nullprogram.com/blog/2018/07/31/).
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x7feb352du;
+    x ^= x >> 15;
+    x *= 0x846ca68bu;
+    return x ^ (x >> 16);
+}
+
+// |value| <= 448 on one of the two e4m3 numbers around it: the larger one when the cut part exceeds `dither` / 2^16.
+// NaN stays NaN: every comparison with it is false, and floorf hands it on.
+__device__ __forceinline__ float round_e4m3(float value, uint32_t dither) {
+    float a = fabsf(value);
+    if (a > kE4m3Max) a = kE4m3Max;
+    const float normal = __uint_as_float((__float_as_uint(a) + (dither << 4)) & 0xfff00000u);
+    const float small = floorf(a * 512.f + static_cast<float>(dither) * (1.f / 65536.f)) * (1.f / 512.f);
+    return copysignf(a >= 0.015625f ? normal : small, value);
+}
+
+template <typename T> __device__ __forceinline__ void load8(float (&to)[8], const T* from, int64_t left, bool wide) {
+    if (wide && left >= 8) {
+        constexpr int kVectors = 8 * sizeof(T) / 16;
+        union { uint4 vector[kVectors]; T element[8]; } u;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) u.vector[i] = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = to_float(u.element[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = i < left ? to_float(from[i]) : 0.f;
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store8(T* to, const float (&from)[8], int64_t left, bool wide) {
+    if (wide && left >= 8) {
+        constexpr int kVectors = 8 * sizeof(T) / 16;
+        union { uint4 vector[kVectors]; T element[8]; } u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u.element[i] = from_float<T>(from[i]);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) __stcs(reinterpret_cast<uint4*>(to) + i, u.vector[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) to[i] = from_float<T>(from[i]);
+    }
+}
+
+__device__ __forceinline__ void decode8(float (&to)[8], uint2 codes, float scale) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t byte = ((i < 4 ? codes.x : codes.y) >> (8 * (i % 4))) & 0xff;
+        const __half_raw half = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
+        to[i] = __fmul_rn(__half2float(__half(half)), scale);
+    }
+}
+
+__device__ __forceinline__ uint2 encode8(const float (&from)[8]) {
+    uint32_t word[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(from[i], from[i + 1]), __NV_SATFINITE, __NV_E4M3);
+        word[i / 4] |= two << (8 * (i % 4));
+    }
+    return make_uint2(word[0], word[1]);
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int step = 16; step; step >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, step));
+    return x;
+}
+
+template <typename P, typename G, int BITS, int CAPACITY>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Args<CAPACITY> a) {
+    const float scale = a.scale_at ? *a.scale_at : 1.f;
+    if (!(fabsf(scale) <= 3.402823466e38f)) return;                    // not finite: this step does not happen
+    const int64_t step = a.state.steps[blockIdx.x] + 1;
+    const float lr = a.lr_at ? *a.lr_at : a.lr;
+    // 1 - b^t without cancellation
+    const float left1 = -expm1f(static_cast<float>(static_cast<double>(step) * a.log_beta1));
+    const float left2 = -expm1f(static_cast<float>(static_cast<double>(step) * a.log_beta2));
+    const float pace = lr / left1, spread = 1.f / sqrtf(left2);
+    const uint32_t salt = mix(static_cast<uint32_t>(step) + a.seed * 0x9e3779b9u);
+
+    // Each block takes a contiguous run of chunks, so it searches for its first tensor once and walks on from there.
+    const int begin = static_cast<int>(static_cast<int64_t>(a.chunks) * blockIdx.x / gridDim.x);
+    const int end = static_cast<int>(static_cast<int64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
+    int low = 0, high = a.count - 1;
+    while (low < high) {
+        const int middle = (low + high + 1) / 2;
+        if (a.items[middle].first_chunk <= begin) low = middle;
+        else high = middle - 1;
+    }
+    int which = low;
+    for (int chunk = begin; chunk < end; ++chunk) {
+        while (which + 1 < a.count && a.items[which + 1].first_chunk <= chunk) ++which;
+        const Item& item = a.items[which];
+        const int64_t at = static_cast<int64_t>(chunk - item.first_chunk) * kChunk + threadIdx.x * kPerThread;
+        const int64_t left = item.count - at;
+        const int64_t flat = item.offset + at;
+        P* param = static_cast<P*>(item.param) + at;
+        const G* grad = static_cast<const G*>(item.grad) + at;
+        const bool wide_param = reinterpret_cast<uintptr_t>(item.param) % 16 == 0, wide_grad = reinterpret_cast<uintptr_t>(item.grad) % 16 == 0;
+        float p[8], g[8], m[8] = {}, v[8] = {};
+        // Lanes behind the tensor's end stay in the warp for the block maximum; their values are zeros.
+        const bool inside = left > 0;
+        uint2 mean_codes = make_uint2(0, 0), root_codes = make_uint2(0, 0);
+        float mean_scale = 0.f, root_scale = 0.f;
+        const int64_t block = flat / TK_ADAMW_BLOCK;
+        const bool block_inside = item.count - (at - (threadIdx.x % 32) * kPerThread) > 0;
+        if (BITS == 8) {
+            if (block_inside) {
+                mean_scale = a.state.mean_scale[block];
+                root_scale = a.state.root_scale[block];
+                mean_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.state.mean) + flat));
+                root_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.state.square) + flat));
+            }
+        }
+        load8<P>(p, param, left, wide_param);
+        load8<G>(g, grad, left, wide_grad);
+        if (BITS == 8) {
+            decode8(m, mean_codes, mean_scale);
+            decode8(v, root_codes, root_scale);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+        } else {
+            // the flat state is padded to whole blocks, so it is always read and written whole
+            if (inside) {
+                load8<float>(m, static_cast<const float*>(a.state.mean) + flat, 8, true);
+                load8<float>(v, static_cast<const float*>(a.state.square) + flat, 8, true);
+            }
+        }
+        const float decay = 1.f - lr * item.weight_decay;
+        float top_mean = 0.f, top_root = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float gradient = i < left ? __fmul_rn(g[i], scale) : 0.f;
+            m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.one_minus_beta1, gradient));
+            v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(__fmul_rn(a.one_minus_beta2, gradient), gradient));
+            const float root = sqrtf(v[i]);
+            p[i] = p[i] * decay - pace * m[i] / (root * spread + a.eps);
+            if (BITS == 8) {
+                v[i] = root;
+                if (i < left) {
+                    top_mean = fmaxf(top_mean, fabsf(m[i]));
+                    top_root = fmaxf(top_root, root);
+                }
+            }
+        }
+        store8<P>(param, p, left, wide_param);
+        if (BITS == 8) {
+            top_mean = warp_max(top_mean);
+            top_root = warp_max(top_root);
+            if (block_inside) {
+                const float mean_factor = top_mean >= kSmallest ? __fmul_rn(__frcp_rn(top_mean), kE4m3Max) : 0.f;
+                const float root_factor = top_root >= kSmallest ? __fmul_rn(__frcp_rn(top_root), kE4m3Max) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t random = mix(static_cast<uint32_t>(flat + i) ^ salt);
+                    const float root = v[i];
+                    m[i] = i < left ? round_e4m3(__fmul_rn(m[i], mean_factor), random & 0xffff) : 0.f;
+                    v[i] = i < left ? round_e4m3(__fmul_rn(root, root_factor), random >> 16) : 0.f;
+                    if (i < left && root > 0.f && v[i] < 1.f / 512.f) v[i] = 1.f / 512.f;
+                }
+                __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.state.mean) + flat), encode8(m));
+                __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.state.square) + flat), encode8(v));
+                if (threadIdx.x % 32 == 0) {
+                    a.state.mean_scale[block] = top_mean >= kSmallest ? __fmul_rn(top_mean, 1.f / kE4m3Max) : 0.f;
+                    a.state.root_scale[block] = top_root >= kSmallest ? __fmul_rn(top_root, 1.f / kE4m3Max) : 0.f;
+                }
+            }
+        } else if (inside) {
+            store8<float>(static_cast<float*>(a.state.mean) + flat, m, 8, true);
+            store8<float>(static_cast<float*>(a.state.square) + flat, v, 8, true);
+        }
+    }
+    // Only this block reads the counters it advances, so no block can see another's new value.
+    if (a.last)
+        for (int i = blockIdx.x + gridDim.x * threadIdx.x; i < TK_ADAMW_COUNTERS; i += gridDim.x * kThreads) {
+            if (i == blockIdx.x) continue;
+            a.state.steps[i] = step;
+        }
+    __syncthreads();
+    if (a.last && threadIdx.x == 0) a.state.steps[blockIdx.x] = step;
+}
+
+template <typename P, typename G, int BITS, int CAPACITY>
+int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+    Args<CAPACITY> a;
+    a.state = *state;
+    a.lr_at = o->lr_at;
+    a.scale_at = o->scale_at;
+    a.log_beta1 = log(o->beta1);
+    a.log_beta2 = log(o->beta2);
+    a.lr = static_cast<float>(o->lr);
+    a.beta1 = static_cast<float>(o->beta1);
+    a.beta2 = static_cast<float>(o->beta2);
+    a.one_minus_beta1 = static_cast<float>(1.0 - o->beta1);
+    a.one_minus_beta2 = static_cast<float>(1.0 - o->beta2);
+    a.eps = static_cast<float>(o->eps);
+    a.seed = o->seed;
+    a.count = count;
+    a.last = last;
+    int64_t chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        a.items[i] = {tensors[i].param, tensors[i].grad, tensors[i].offset, tensors[i].count, static_cast<int32_t>(chunks), tensors[i].weight_decay};
+        chunks += (tensors[i].count + kChunk - 1) / kChunk;
+        if (chunks > 0x7fffffff) return fail(TK_E_ARGUMENT, "trainkernel: too many elements in one tk_adamw_update");
+    }
+    a.chunks = static_cast<int32_t>(chunks);
+    int64_t grid = static_cast<int64_t>(sms) * 8;
+    if (grid > TK_ADAMW_COUNTERS) grid = TK_ADAMW_COUNTERS;
+    if (grid > chunks) grid = chunks;
+    if (grid < 1) grid = 1;
+    adamw_kernel<P, G, BITS, CAPACITY><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a);
+    count_launch();
+    return check(cudaGetLastError(), "launching the AdamW kernel");
+}
+
+template <typename P, typename G, int BITS>
+int launch_all(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+    while (count > kMany) {
+        if (int code = launch<P, G, BITS, kMany>(tensors, kMany, state, o, 0, sms, stream)) return code;
+        tensors += kMany;
+        count -= kMany;
+    }
+    return count > kFew ? launch<P, G, BITS, kMany>(tensors, count, state, o, last, sms, stream)
+                        : launch<P, G, BITS, kFew>(tensors, count, state, o, last, sms, stream);
+}
+
+template <typename P, typename G>
+int by_bits(const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+    return o->bits == 8 ? launch_all<P, G, 8>(t, n, s, o, last, sms, stream) : launch_all<P, G, 32>(t, n, s, o, last, sms, stream);
+}
+
+template <typename P>
+int by_grad(int dtype, const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+    switch (dtype) {
+        case TK_F32: return by_bits<P, float>(t, n, s, o, last, sms, stream);
+        case TK_F16: return by_bits<P, __half>(t, n, s, o, last, sms, stream);
+        default: return by_bits<P, __nv_bfloat16>(t, n, s, o, last, sms, stream);
+    }
+}
+
+}  // namespace
+
+extern "C" int tk_adamw_update(const tk_adamw_tensor* tensors, int count, int param_dtype, int grad_dtype, const tk_adamw_state* state,
+                               const tk_adamw_options* options, int last, int device, void* stream) {
+    if (!tensors || count < 1 || !state || !options || !state->mean || !state->square || !state->steps || param_dtype < TK_F32
+        || param_dtype > TK_BF16 || grad_dtype < TK_F32 || grad_dtype > TK_BF16 || (options->bits != 8 && options->bits != 32)
+        || (options->bits == 8 && (!state->mean_scale || !state->root_scale)) || !(options->beta1 >= 0 && options->beta1 < 1)
+        || !(options->beta2 >= 0 && options->beta2 < 1))
+        return fail(TK_E_ARGUMENT, "trainkernel: invalid argument to tk_adamw_update");
+    for (int i = 0; i < count; ++i)
+        if (tensors[i].count < 0 || tensors[i].offset < 0 || tensors[i].offset % TK_ADAMW_BLOCK
+            || (tensors[i].count && (!tensors[i].param || !tensors[i].grad)))
+            return fail(TK_E_ARGUMENT, "trainkernel: invalid tensor %d passed to tk_adamw_update", i);
+    DeviceScope scope(device);
+    if (scope.status) return scope.status;
+    const int sms = tk_ops::sm_count(device);
+    if (sms < 1) return fail(TK_E_ARGUMENT, "trainkernel: device %d cannot be asked for its multiprocessors", device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (param_dtype) {
+        case TK_F32: return by_grad<float>(grad_dtype, tensors, count, state, options, last, sms, s);
+        case TK_F16: return by_grad<__half>(grad_dtype, tensors, count, state, options, last, sms, s);
+        default: return by_grad<__nv_bfloat16>(grad_dtype, tensors, count, state, options, last, sms, s);
+    }
+}
