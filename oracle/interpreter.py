@@ -69,6 +69,86 @@ _EAGER["eq"] = lambda op, a: torch.eq(a[0], a[1])
 _EAGER["arange"] = lambda op, a: torch.arange(op.attrs["end"])
 
 
+# -- the package's own operators (not in the reference), in FP64 from their definitions ------------------------
+
+def _rows(logits, targets, mask):
+    keep = torch.ones_like(targets, dtype=torch.bool) if mask is None else mask
+    x = torch.where(keep.unsqueeze(-1), logits, torch.zeros_like(logits)).double()
+    top = x.amax(-1)
+    total = torch.exp(x - top.unsqueeze(-1)).sum(-1)
+    logp = x.gather(-1, targets.long().unsqueeze(-1)).squeeze(-1) - top - torch.log(total)
+    return x, keep, torch.where(keep, logp, torch.zeros_like(logp)), torch.stack((top, total), -1)
+
+
+def _logits_grad(logits, targets, mask, coefficients, stats, scale):
+    x, keep, _, _ = _rows(logits, targets, mask)
+    if coefficients.dim() < targets.dim():
+        coefficients = coefficients.unsqueeze(-1)
+    c = torch.where(keep, coefficients.double().expand(targets.shape), 0.0) * (1.0 if scale is None else float(scale))
+    hot = torch.zeros_like(x).scatter_(-1, targets.long().unsqueeze(-1), 1.0)
+    return c.unsqueeze(-1) * (hot - torch.softmax(x, -1))
+
+
+def _policy(logits, targets, old, advantages, ref, mask, low, high, kl_weight, average):
+    _, keep, logp, stats = _rows(logits, targets, mask)
+    ratio = torch.exp(logp - old.double())
+    free, bound = ratio * advantages, ratio.clamp(1 - low, 1 + high) * advantages
+    term, slope = -torch.minimum(free, bound), torch.where(free <= bound, -free, torch.zeros_like(free))
+    if ref is not None:
+        away = ref.double() - logp
+        term, slope = term + kl_weight * (torch.exp(away) - away - 1), slope + kl_weight * (1 - torch.exp(away))
+    weight = keep.double()
+    if average == 0 or targets.dim() == 1:
+        weight = weight / keep.sum().clamp(min=1)
+    else:
+        weight = weight / (keep.sum(1, keepdim=True).clamp(min=1) * targets.shape[0])
+    zero = torch.zeros_like(term)
+    return torch.where(keep, weight * term, zero).sum(), logp, stats, torch.where(keep, weight * slope, zero)
+
+
+def _preference(logits, targets, reference, mask, beta, smoothing):
+    _, _, logp, stats = _rows(logits, targets, mask)
+    sums = logp.sum(1)
+    margin = sums - reference.double()
+    n = sums.shape[0] // 2
+    z = beta * (margin[:n] - margin[n:])
+    logsig = torch.nn.functional.logsigmoid
+    loss = (-(1 - smoothing) * logsig(z) - smoothing * logsig(-z)).mean()
+    slope = beta / n * (smoothing * torch.sigmoid(z) - (1 - smoothing) * torch.sigmoid(-z))
+    return loss, sums, stats, torch.cat((slope, -slope))
+
+
+def _policy_and_grad(logits, targets, *rest):
+    loss, logp, stats, slope = _policy(logits, targets, *rest[:-1])
+    return loss, logp, _logits_grad(logits, targets, rest[3], slope, stats, rest[-1])
+
+
+def _preference_and_grad(logits, targets, reference, mask, beta, smoothing, scale):
+    loss, sums, stats, slope = _preference(logits, targets, reference, mask, beta, smoothing)
+    return loss, sums, _logits_grad(logits, targets, mask, slope, stats, scale)
+
+
+_OPERATORS = {
+    "token_logprobs": lambda logits, targets, mask: _rows(logits, targets, mask)[2:],
+    "token_logprobs_and_grad": lambda logits, targets, weights, mask, scale: (_rows(logits, targets, mask)[2],
+                                                                              _logits_grad(logits, targets, mask, weights, None, scale)),
+    "token_logits_grad": lambda *a: (_logits_grad(*a),),
+    "policy_loss": _policy,
+    "policy_loss_and_grad": _policy_and_grad,
+    "preference_loss": _preference,
+    "preference_loss_and_grad": _preference_and_grad,
+}
+
+
+def _operator(op: Operation, operands: list) -> torch.Tensor:
+    arguments = [operands[value] if kind == "operand" else value for kind, value in op.attrs["arguments"]]
+    return _OPERATORS[op.op](*arguments)[op.attrs["result"]]
+
+
+for _name in _OPERATORS:
+    _EAGER[_name] = _operator
+
+
 def run(program: Program, inputs: Sequence[torch.Tensor]) -> tuple[torch.Tensor, ...]:
     """Evaluate `program` on `inputs`; returns one tensor per program output."""
     if len(inputs) != len(program.inputs):

@@ -11,6 +11,7 @@ reference's.
 """
 from __future__ import annotations
 
+import operator
 from collections.abc import Callable, Sequence
 from dataclasses import dataclass
 from typing import Any, Generic, TypeVar
@@ -28,6 +29,9 @@ DTYPE_NAMES = {torch.float32: "float32", torch.float16: "float16", torch.bfloat1
 # and benchmarks/train_loop.py:66-68).  Index dtypes may only flow through arange / eq / casts.
 INDEX_DTYPE_NAMES = {torch.int64: "int64", torch.int32: "int32", torch.bool: "bool"}
 _INDEX_OPS = ("arange", "eq", "cast")
+# Calls of the package's own operators (`losses.py`) are recorded whole, under the operator's name: one IR operation per
+# result that is used, all of them with the same `call`.  They run between generated kernels, not inside one.
+OPERATOR_NAMESPACE = "trainkernel."
 
 _PERMUTING = ("aten.t.default", "aten.transpose.int", "aten.permute.default")
 _IDENTITY_VIEWS = ("aten.alias.default", "aten.detach.default")
@@ -90,14 +94,16 @@ class CompiledFunction(Generic[R]):
         leaves = self._flatten_inputs(args)
         self.runner._validate_inputs(leaves)
         device = self.runner.device
-        targets = sorted(set(self.runner.inplace_outputs.values()))
+        # what a call changes: the in-place targets, and what the runner itself keeps (optimizer moments)
+        targets = [leaves[index] for index in sorted(set(self.runner.inplace_outputs.values()))]
+        targets += getattr(self.runner, "kept_tensors", ())
 
-        def restore(snapshot: dict[int, torch.Tensor]) -> None:
-            for index, saved in snapshot.items():
-                leaves[index].copy_(saved)
+        def restore(snapshot: list[torch.Tensor]) -> None:
+            for target, saved in zip(targets, snapshot):
+                target.copy_(saved)
 
         with torch.cuda.device(device):
-            snapshot = {index: leaves[index].clone() for index in targets}
+            snapshot = [target.clone() for target in targets]
             try:
                 for _ in range(warmup):
                     self(*args)
@@ -222,6 +228,22 @@ def _lower_call(node: torch.fx.Node, specs: dict[torch.fx.Node, TensorSpec]) -> 
     raise ValueError(f"trainkernel: unsupported ATen op {target} at {node.name}")
 
 
+def _lower_operator(node: torch.fx.Node, specs: dict[torch.fx.Node, TensorSpec]) -> tuple[str, tuple, dict[str, object]]:
+    """`(ir_op, tensor operands, attrs)` of a call of one of the package's operators.
+
+    `attrs["arguments"]` rebuilds the call: `("operand", k)` stands for operand k, `("value", v)` for a number or None.
+    """
+    operands: list[TensorSpec] = []
+    arguments: list[tuple[str, object]] = []
+    for arg in node.args:
+        if isinstance(arg, torch.fx.Node):
+            arguments.append(("operand", len(operands)))
+            operands.append(specs[arg])
+        else:
+            arguments.append(("value", arg))
+    return str(node.target).split(".")[1], tuple(operands), {"arguments": tuple(arguments), "call": node.name}
+
+
 def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Program, TreeSpec]:
     """Trace a pure function of tensor pytrees into a `Program`.
 
@@ -233,8 +255,8 @@ def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Prog
     leaves, input_tree = tree_flatten(tuple(example_inputs))
     if not leaves or not all(isinstance(leaf, torch.Tensor) for leaf in leaves):
         raise TypeError("trainkernel: example_inputs must contain tensors only and cannot be empty")
-    if not all(leaf.dtype in DTYPE_NAMES or leaf.dtype in (torch.int64, torch.int32) for leaf in leaves):
-        raise ValueError("trainkernel: unsupported dtype; expected float32, float16, or bfloat16 (int32/int64 for class labels)")
+    if not all(leaf.dtype in DTYPE_NAMES or leaf.dtype in INDEX_DTYPE_NAMES for leaf in leaves):
+        raise ValueError("trainkernel: unsupported dtype; expected float32, float16, or bfloat16 (int32/int64 for class labels, bool for masks)")
     if not all(leaf.layout == torch.strided for leaf in leaves):
         raise ValueError("trainkernel: only strided tensors are supported")
     if not all(leaf.device == leaves[0].device for leaf in leaves):
@@ -254,8 +276,14 @@ def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Prog
         result_tree[:] = [tree]
         return tuple(out_leaves)
 
+    from .losses import NotFunctional
     try:
-        traced = make_fx(functionalize(on_leaves), tracing_mode="fake", _allow_non_fake_inputs=True)(*leaves)
+        try:
+            traced = make_fx(functionalize(on_leaves), tracing_mode="fake", _allow_non_fake_inputs=True)(*leaves)
+        except NotFunctional:
+            # Without functionalization an in-place operation stays one, and is refused below as any other would be.
+            traced = make_fx(on_leaves, tracing_mode="fake", _allow_non_fake_inputs=True)(*leaves)
+            traced.graph.eliminate_dead_code()
     except Exception as error:
         raise RuntimeError(f"trainkernel: FX capture failed: {error}") from error
 
@@ -264,6 +292,7 @@ def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Prog
     program_inputs: list[TensorSpec] = []
     operations: list[Operation] = []
     returned: list[Any] = []
+    calls: dict[torch.fx.Node, tuple[str, tuple, dict[str, object]]] = {}
     for node in traced.graph.nodes:
         if node.op == "output":
             returned, _ = tree_flatten(node.args[0])
@@ -276,6 +305,9 @@ def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Prog
             target = str(node.target)
             if target.startswith("aten.copy_"):
                 raise ValueError("trainkernel: input mutation is unsupported; return updated tensors instead")
+            if target.startswith(OPERATOR_NAMESPACE) and not isinstance(node.meta.get("val"), torch.Tensor):
+                calls[node] = _lower_operator(node, specs)          # several results: each is picked below
+                continue
             shape, dtype = _node_signature(node)
             if node.meta["val"].device != device:
                 raise ValueError("trainkernel: cross-device operations are unsupported")
@@ -283,7 +315,14 @@ def capture(fn: Callable[..., Any], example_inputs: Sequence[Any]) -> tuple[Prog
                 base = next(specs[arg] for arg in node.args if isinstance(arg, torch.fx.Node))
                 specs[node] = _fold_view(node, base, shape, dtype)
                 continue
-            kind, operands, attrs = _lower_call(node, specs)
+            if node.target is operator.getitem and node.args[0] in calls:
+                kind, operands, attrs = calls[node.args[0]]
+                attrs = {**attrs, "result": int(node.args[1])}
+            elif target.startswith(OPERATOR_NAMESPACE):
+                kind, operands, attrs = _lower_operator(node, specs)
+                attrs["result"] = 0
+            else:
+                kind, operands, attrs = _lower_call(node, specs)
             if dtype in INDEX_DTYPE_NAMES.values() and kind not in _INDEX_OPS:
                 raise ValueError(f"trainkernel: unsupported dtype {node.meta['val'].dtype} at {node.name}; "
                                  "integer tensors may only feed arange / eq / casts (one-hot labels)")
@@ -325,7 +364,32 @@ def _subtrees(tree: TreeSpec) -> Sequence[TreeSpec]:
     return accessor() if callable(accessor) else tree.children_specs
 
 
-def compile_training(fn: Callable[..., Any], example_inputs: Sequence[Any], **options: Any) -> CompiledTrainingStep[Any]:
+def _compile_with_optimizer(fn: Callable[..., Any], example_inputs: Sequence[Any], optimizer: Any, options: dict[str, Any]) -> CompiledTrainingStep[Any]:
+    """`compile_training` of `(state, *data) -> (scalar_loss, gradients)` with an optimizer's update behind the kernel."""
+    from .optim import AdamW
+    if not isinstance(optimizer, AdamW):
+        raise TypeError("trainkernel: optimizer must be an AdamW")
+    program, output_tree = capture(fn, example_inputs)
+    _, input_tree = tree_flatten(tuple(example_inputs))
+    state_tree = _subtrees(input_tree)[0]
+    parts = _subtrees(output_tree)
+    if output_tree.type not in (tuple, list) or len(parts) != 2:
+        raise ValueError("trainkernel: with an optimizer the training function must return loss, gradients")
+    if not parts[0].is_leaf() or parts[1] != state_tree:
+        raise ValueError("trainkernel: gradients must match the state pytree")
+    count = state_tree.num_leaves
+    if count == 0 or program.outputs[0].shape != ():
+        raise ValueError("trainkernel: training requires nonempty state and a scalar loss")
+    for gradient, parameter in zip(program.outputs[1:], program.inputs[:count]):
+        if (gradient.shape, gradient.dtype) != (parameter.shape, parameter.dtype):
+            raise ValueError("trainkernel: gradients must match parameter shapes and dtypes")
+    from . import runtime, segments
+    runner = segments.OptimizedProgram(runtime.compile_program(program, example_inputs, **options), optimizer, tree_flatten(tuple(example_inputs))[0][:count])
+    _, result_tree = tree_flatten((0, *(tree_unflatten([0] * count, state_tree) for _ in range(2))))
+    return CompiledTrainingStep(program, runner, input_tree, result_tree)
+
+
+def compile_training(fn: Callable[..., Any], example_inputs: Sequence[Any], *, optimizer: Any = None, **options: Any) -> CompiledTrainingStep[Any]:
     """Compile `(state, *data) -> (scalar_loss, gradients, updated_state)`.
 
     The gradient and updated-state pytrees must mirror the state pytree.  Each
@@ -333,9 +397,15 @@ def compile_training(fn: Callable[..., Any], example_inputs: Sequence[Any], **op
     directly by the producing stage when the planner proves the old value has
     had its last read, otherwise through a staged copy after a final barrier.
     State tensors must not require grad; differentiation is inside `fn`.
+
+    With `optimizer=AdamW(...)`, `fn` returns `(scalar_loss, gradients)` and the update follows the compiled
+    kernel on the same stream, in place, with moments the compiled step keeps (`step.runner.state`); a captured
+    step advances them with every replay.  Calls return `(loss, gradients, state)` as without one.
     """
     if "inplace_outputs" in options:
         raise ValueError("trainkernel: compile_training derives its own state mapping")
+    if optimizer is not None:
+        return _compile_with_optimizer(fn, example_inputs, optimizer, options)
     program, output_tree = capture(fn, example_inputs)
     _, input_tree = tree_flatten(tuple(example_inputs))
     state_tree = _subtrees(input_tree)[0]

@@ -220,7 +220,7 @@ def _preference_launch(logits, targets, reference, mask, beta: float, smoothing:
 _ops = torch.library.Library("trainkernel", "DEF")
 _ops.define("token_logprobs(Tensor logits, Tensor targets, Tensor? mask) -> (Tensor, Tensor)")
 _ops.define("token_logprobs_and_grad(Tensor logits, Tensor targets, Tensor weights, Tensor? mask, float scale) -> (Tensor, Tensor)")
-_ops.define("token_logits_grad(Tensor logits, Tensor targets, Tensor? mask, Tensor coefficients, Tensor stats, Tensor scale) -> Tensor")
+_ops.define("token_logits_grad(Tensor logits, Tensor targets, Tensor? mask, Tensor coefficients, Tensor stats, Tensor? scale) -> Tensor")
 _ops.define("policy_loss(Tensor logits, Tensor targets, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, Tensor? mask, "
             "float clip_low, float clip_high, float kl_weight, int average) -> (Tensor, Tensor, Tensor, Tensor)")
 _ops.define("policy_loss_and_grad(Tensor logits, Tensor targets, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, Tensor? mask, "
@@ -319,14 +319,16 @@ class _TokenLogprobs(torch.autograd.Function):
     def setup_context(ctx, inputs, output):
         logits, targets, mask = inputs
         ctx.has_mask = mask is not None
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(output[1])
         ctx.save_for_backward(logits, targets, output[1], *([mask] if ctx.has_mask else []))
 
     @staticmethod
     def backward(ctx, grad_logprobs, _):
+        if grad_logprobs is None:
+            return None, None, None
         logits, targets, stats, *mask = ctx.saved_tensors
-        one = torch.ones((), dtype=torch.float32, device=logits.device)
-        return _LogitsGrad.apply(logits, targets, mask[0] if mask else None, grad_logprobs, stats, one), None, None
+        return _LogitsGrad.apply(logits, targets, mask[0] if mask else None, grad_logprobs, stats, None), None, None
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -338,11 +340,14 @@ class _PolicyLoss(torch.autograd.Function):
     def setup_context(ctx, inputs, output):
         logits, targets, mask = inputs[0], inputs[1], inputs[5]
         ctx.has_mask = mask is not None
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*output[1:])
         ctx.save_for_backward(logits, targets, output[2], output[3], *([mask] if ctx.has_mask else []))
 
     @staticmethod
     def backward(ctx, grad_loss, *_):
+        if grad_loss is None:
+            return (None,) * 10
         logits, targets, stats, coefficients, *mask = ctx.saved_tensors
         grad = _LogitsGrad.apply(logits, targets, mask[0] if mask else None, coefficients, stats, grad_loss)
         return (grad, *(None,) * 9)
@@ -357,14 +362,29 @@ class _PreferenceLoss(torch.autograd.Function):
     def setup_context(ctx, inputs, output):
         logits, targets, mask = inputs[0], inputs[1], inputs[3]
         ctx.has_mask = mask is not None
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*output[1:])
         ctx.save_for_backward(logits, targets, output[2], output[3], *([mask] if ctx.has_mask else []))
 
     @staticmethod
     def backward(ctx, grad_loss, *_):
+        if grad_loss is None:
+            return (None,) * 6
         logits, targets, stats, coefficients, *mask = ctx.saved_tensors
         grad = _LogitsGrad.apply(logits, targets, mask[0] if mask else None, coefficients, stats, grad_loss)
         return (grad, *(None,) * 5)
+
+
+class NotFunctional(Exception):
+    """Raised inside a functionalized trace: functionalization has no rule for a differentiable operator of this module,
+    so `capture` traces such a function once more without it (nothing these operators do needs it)."""
+
+
+def _differentiable(function: type[torch.autograd.Function], *args):
+    stack = torch._C._functorch.peek_interpreter_stack()
+    if stack is not None and any(level.key() == torch._C._functorch.TransformType.Functionalize for level in torch._C._functorch.get_interpreter_stack()):
+        raise NotFunctional
+    return function.apply(*args)
 
 
 def _is_plain(logits: torch.Tensor) -> bool:
@@ -393,7 +413,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, mask: torch.T
     _check_rows("token_logprobs", logits, targets, mask)
     if _is_plain(logits) and not _records("token_logprobs", logits):
         return _logprobs_launch(logits, targets, mask, False)[0]
-    return _TokenLogprobs.apply(logits, targets, mask)[0]
+    return _differentiable(_TokenLogprobs, logits, targets, mask)[0]
 
 
 def token_logprobs_and_grad(logits: torch.Tensor, targets: torch.Tensor, weights: torch.Tensor, *, mask: torch.Tensor | None = None,
@@ -427,7 +447,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
     old, advantages, ref, low, high, kl_weight, which = _check_policy(who, logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip, kl_weight, average)
     if _is_plain(logits) and not _records(who, logits):
         return _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_weight, which, saved=False, grad=False)[:2]
-    return _PolicyLoss.apply(logits, targets, old, advantages, ref, mask, low, high, kl_weight, which)[:2]
+    return _differentiable(_PolicyLoss, logits, targets, old, advantages, ref, mask, low, high, kl_weight, which)[:2]
 
 
 def policy_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
@@ -467,7 +487,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: torc
     reference, beta, label_smoothing = _check_preference(who, logits, targets, reference, mask, beta, label_smoothing)
     if _is_plain(logits) and not _records(who, logits):
         return _preference_launch(logits, targets, reference, mask, beta, label_smoothing, grad=False)[:2]
-    return _PreferenceLoss.apply(logits, targets, reference, mask, beta, label_smoothing)[:2]
+    return _differentiable(_PreferenceLoss, logits, targets, reference, mask, beta, label_smoothing)[:2]
 
 
 def preference_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, reference: torch.Tensor, *, mask: torch.Tensor | None = None,

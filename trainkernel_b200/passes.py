@@ -247,3 +247,62 @@ def insert_gradient_exchange(program: Program, state_count: int) -> Program:
             result = TensorSpec(name, op.output.shape, op.output.dtype, row_major(op.output.shape), name)
             operations.append(Operation(name, "allreduce", (op.output,), result, {}))
     return Program(program.inputs, tuple(operations), tuple(redirect(v) for v in program.outputs))
+
+
+_LOSS_RESULTS = {"policy_loss": (2, 3), "preference_loss": (2, 3)}       # results that only the backward operation needs
+
+
+def fuse_loss_gradients(program: Program) -> Program:
+    """Merge a loss operator with the operation that differentiates it, so that the logits are read once.
+
+    Differentiating `policy_loss` or `preference_loss` leaves two operations: the loss, which also returns the rows'
+    statistics and coefficients, and `token_logits_grad`, which reads the logits again.  When the gradient that
+    arrives at the loss is a constant (the loss of a training step is not used any further) and nobody else reads
+    statistics and coefficients, both become the operator's `_and_grad` form with that constant as its scale.
+    """
+    producer = {op.output.buffer: op for op in program.operations}
+    merged: dict[str, tuple[Operation, float]] = {}               # loss call -> (backward operation, scale)
+    for op in program.operations:
+        if op.op != "token_logits_grad":
+            continue
+        arguments = op.attrs["arguments"]
+        operands = [op.inputs[value] if kind == "operand" else value for kind, value in arguments]
+        logits, targets, mask, coefficients, stats, scale = operands
+        loss = producer.get(stats.buffer)
+        fill = None if scale is None else producer.get(scale.buffer)
+        if loss is None or loss.op not in _LOSS_RESULTS or fill is None or fill.op != "full":
+            continue
+        call = loss.attrs["call"]
+        parts = [other for other in program.operations if other.attrs.get("call") == call]
+        hidden = {other.output.buffer: other for other in parts if other.attrs["result"] in _LOSS_RESULTS[loss.op]}
+        both = producer.get(coefficients.buffer)
+        if both is None or both.attrs.get("call") != call or {stats.buffer, coefficients.buffer} != set(hidden):
+            continue
+        if not all(value.strides == row_major(value.shape) and value.offset == 0 for value in (stats, coefficients)):
+            continue
+        if any(len(_uses_of(program, buffer)) != 1 for buffer in hidden):
+            continue
+        before = [loss.inputs[value] if kind == "operand" else value for kind, value in loss.attrs["arguments"]]
+        same = (before[0], before[1], before[5 if loss.op == "policy_loss" else 3]) == (logits, targets, mask)
+        if same and call not in merged:
+            merged[call] = (op, float(fill.attrs["value"]))
+    if not merged:
+        return program
+    backward = {op.output.buffer: call for call, (op, _) in merged.items()}
+    operations: list[Operation] = []
+    seen: set[str] = set()
+    for op in program.operations:
+        call = op.attrs.get("call")
+        if op.output.buffer in backward:
+            continue
+        if call not in merged:
+            operations.append(op)
+            continue
+        gradient, scale = merged[call]
+        attrs = {**op.attrs, "arguments": (*op.attrs["arguments"], ("value", scale))}
+        if call not in seen:
+            seen.add(call)
+            operations.append(replace(gradient, op=op.op + "_and_grad", inputs=op.inputs, attrs={**attrs, "result": 2}))
+        if op.attrs["result"] not in _LOSS_RESULTS[op.op]:
+            operations.append(replace(op, op=op.op + "_and_grad", attrs=attrs))
+    return Program(program.inputs, tuple(operations), program.outputs)

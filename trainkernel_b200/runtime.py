@@ -471,7 +471,11 @@ class CompiledProgram:
 def compile_program(program: Program, example_inputs: tuple[Any, ...] | list[Any], *,
                     inplace_outputs: dict[int, int] | None = None, verbose: bool = False,
                     **options: Any) -> CompiledProgram:
-    """Generate, build and load the kernel for `program` on the inputs' device (sm_100 required)."""
+    """Generate, build and load the kernel for `program` on the inputs' device (sm_100 required).
+
+    A program that calls the package's own operators (`losses.py`) becomes a `segments.SegmentedProgram`:
+    generated kernels with the operators' launches between them, behind the same call interface.
+    """
     flat, _ = tree_flatten(example_inputs)
     if not flat or any(not isinstance(x, torch.Tensor) for x in flat):
         raise TypeError("trainkernel: nonempty tensor inputs required")
@@ -485,6 +489,9 @@ def compile_program(program: Program, example_inputs: tuple[Any, ...] | list[Any
     capability = torch.cuda.get_device_capability(device)
     if capability[0] != 10:
         raise RuntimeError(f"trainkernel: an sm_100 (B200-class) GPU is required, found compute capability {capability[0]}.{capability[1]}")
+    from . import segments
+    if segments.has_operators(program):
+        return segments.compile_segments(program, flat, inplace_outputs=inplace_outputs, verbose=verbose, **options)
     if "assume_aligned" not in options and any(x.data_ptr() % 16 for x in flat):
         options["assume_aligned"] = False     # example tensors at odd offsets: keep the element-wise fallbacks
     generated = generate(program, inplace_outputs=inplace_outputs, **options)
