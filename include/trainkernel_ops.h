@@ -46,10 +46,12 @@ typedef struct {
     tk_token_array mask;                  /* bytes; data may be NULL: every row counts */
 } tk_token_rows;
 
-/* Where the gradient of the logits goes and what scales it; data NULL: no gradient.  Dense [batch, length, vocab]
- * of the logits' type.  `scale` is multiplied by the FP32 value at `scale_at` when that is not NULL. */
+/* Where the gradient of the logits goes and what scales it; data NULL: no gradient.  Rows of the logits' type with unit
+ * stride inside a row; rows that do not lie as their logits do relative to 16-byte boundaries are written element by
+ * element.  `scale` is multiplied by the FP32 value at `scale_at` when that is not NULL. */
 typedef struct {
     void* data;
+    int64_t stride_batch, stride_token;   /* elements */
     const float* scale_at;
     float scale;
     int32_t reserved;

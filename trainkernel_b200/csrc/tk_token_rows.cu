@@ -20,9 +20,9 @@ using tk_ops::count_launch;
 using tk_ops::DeviceScope;
 using tk_ops::fail;
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kThreads = 512;
+constexpr float kExtreme = 1e38f;                  // beyond it logit * log2(e) may leave FP32's range
 
 // 2^x by the hardware's approximation (relative error about 2^-22).
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -31,21 +31,164 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+// Two FP32 numbers in one 64-bit register, for the paired arithmetic instructions.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 16 bytes of logits.
+template <typename T> struct Vector;
+template <> struct Vector<float> {
+    static constexpr int kCount = 4;
+    static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[2]) {
+        f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+    static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
+        return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    static __device__ __forceinline__ float load(float x) { return x; }
+    static __device__ __forceinline__ float store(float x) { return x; }
+};
+template <> struct Vector<__nv_bfloat16> {
+    static constexpr int kCount = 8;
+    static __device__ __forceinline__ float2 two(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
+        f[0] = two(v.x);
+        f[1] = two(v.y);
+        f[2] = two(v.z);
+        f[3] = two(v.w);
+    }
+    static __device__ __forceinline__ uint32_t word(float2 f) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(f);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) { return make_uint4(word(f[0]), word(f[1]), word(f[2]), word(f[3])); }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+        return fmaxf(f.x, f.y);
+    }
+    static __device__ __forceinline__ float load(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 store(float x) { return __float2bfloat16_rn(x); }
+};
+template <> struct Vector<__half> {
+    static constexpr int kCount = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __half22float2(h[i]);
+    }
+    static __device__ __forceinline__ uint32_t word(float2 f) {
+        const __half2 h = __float22half2_rn(f);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) { return make_uint4(word(f[0]), word(f[1]), word(f[2]), word(f[3])); }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+        const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+        return fmaxf(f.x, f.y);
+    }
+    static __device__ __forceinline__ float load(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half store(float x) { return __float2half_rn(x); }
+};
+
+// x log2(e), rounded on its own (never contracted into a fused operation with what follows).
+__device__ __forceinline__ float scaled(float x) {
+    float y;
+    asm("mul.rn.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(kLog2e));
+    return y;
+}
+
+// The exponent of 2 that stands for exp(x - top): x log2(e) - rn(top log2(e)) in one fused operation.  The rounding of
+// the subtrahend is the same for every logit of the row and for its target, so it cancels.  Where the product could
+// overflow (logits of the type's lowest value everywhere) the difference is taken first.
+struct Exponent {
+    float top, base;
+    bool extreme;
+    __device__ __forceinline__ explicit Exponent(float t) : top(t), base(scaled(t)), extreme(fabsf(t) > kExtreme) {}
+    __device__ __forceinline__ float operator()(float x) const { return extreme ? (x - top) * kLog2e : fmaf(x, kLog2e, -base); }
+};
 
 struct Stat {
-    float top, sum;
+    float top, sum;                        // sum of 2^Exponent(top)(x)
 };
 
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float top = fmaxf(a.top, b.top);
-    return {top, a.sum * exp2_fast((a.top - top) * kLog2e) + b.sum * exp2_fast((b.top - top) * kLog2e)};
+    const Exponent e(top);
+    // A part's sum is relative to its own rounded base, so the bases are what is subtracted, each rounded as it was used.
+    const float x = e.extreme ? (a.top - top) * kLog2e : scaled(a.top) - e.base;
+    const float y = e.extreme ? (b.top - top) * kLog2e : scaled(b.top) - e.base;
+    return {top, a.sum * exp2_fast(x) + b.sum * exp2_fast(y)};
+}
+
+// Adds N vectors of logits to a thread's statistics.
+template <typename T, int N>
+__device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
+    constexpr int kPairs = Vector<T>::kCount / 2;
+    float top = s.top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, Vector<T>::top(v[i]));
+    const Exponent e(top);
+    if (top > s.top) s = join(s, {top, 0.f});
+    if (!e.extreme) {
+        const Pair scale = pair(kLog2e, kLog2e), base = pair(-e.base, -e.base);
+        Pair sum = pair(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float2 f[kPairs];
+            Vector<T>::unpack(v[i], f);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 x = both(fma2(pair(f[k].x, f[k].y), scale, base));
+                sum = add2(sum, pair(exp2_fast(x.x), exp2_fast(x.y)));
+            }
+        }
+        const float2 total = both(sum);
+        s.sum += total.x + total.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float2 f[kPairs];
+            Vector<T>::unpack(v[i], f);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) s.sum += exp2_fast(e(f[k].x)) + exp2_fast(e(f[k].y));
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void accumulate_one(Stat& s, T value) {
+    const float x = Vector<T>::load(value);
+    if (x > s.top) s = join(s, {x, 0.f});
+    s.sum += exp2_fast(Exponent(s.top)(x));
 }
 
 enum Mode { kStats, kGrad, kBoth };            // log-probabilities / gradient from saved stats / both
@@ -55,12 +198,11 @@ struct Args {
     tk_token_rows rows;
     tk_token_array coefficients;               // kGrad and kBoth with kWeights: FP32 [batch, length]
     tk_policy_terms policy;
+    tk_token_grad grad;
     float* logprobs;
     float* stats;
     float* row_coefficients;                   // kPolicy: dense d loss / d logprob, or NULL
-    void* grad;
-    const float* scale_at;
-    float scale;
+    bool in_phase;                             // every row of the gradient lies as its logits do within 16 bytes
     // kPolicy: workspace
     unsigned* counter;
     float* weights;                            // one per sequence
@@ -82,6 +224,7 @@ __device__ __forceinline__ float at(const tk_token_array& a, int64_t b, int64_t 
     return static_cast<const float*>(a.data)[b * a.stride_batch + t * a.stride_token];
 }
 
+template <int THREADS>
 __device__ Stat block_join(Stat mine, Stat* shared) {
 #pragma unroll
     for (int step = 16; step; step >>= 1)
@@ -89,7 +232,7 @@ __device__ Stat block_join(Stat mine, Stat* shared) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (lane == 0) shared[warp] = mine;
     __syncthreads();
-    mine = lane < kThreads / 32 ? shared[lane] : Stat{kLowest, 0.f};
+    mine = lane < THREADS / 32 ? shared[lane] : Stat{kLowest, 0.f};
 #pragma unroll
     for (int step = 16; step; step >>= 1)
         mine = join(mine, {__shfl_xor_sync(~0u, mine.top, step), __shfl_xor_sync(~0u, mine.sum, step)});
@@ -112,36 +255,125 @@ __device__ __forceinline__ void policy_token(const tk_policy_terms& p, int64_t b
     }
 }
 
-template <typename T, Mode MODE, Loss LOSS>
-__global__ void __launch_bounds__(kThreads) token_rows_kernel(const __grid_constant__ Args a) {
+// A row's parts: elements before the first 16-byte boundary, whole vectors, elements behind the last.
+struct Parts {
+    int head, vectors, tail;
+};
+template <typename T>
+__device__ __forceinline__ Parts parts_of(const T* x, int vocab) {
+    constexpr int kCount = Vector<T>::kCount;
+    int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T));
+    head = head < vocab ? head : vocab;
+    return {head, (vocab - head) / kCount, (vocab - head) % kCount};
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ Stat row_stat(const T* x, int vocab) {
+    constexpr int kAhead = 4;                  // vectors a thread has in flight
+    const Parts p = parts_of(x, vocab);
+    const uint4* body = reinterpret_cast<const uint4*>(x + p.head);
+    Stat s{kLowest, 0.f};
+    int i = threadIdx.x;
+    for (; i + (kAhead - 1) * THREADS < p.vectors; i += kAhead * THREADS) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = __ldcg(body + i + k * THREADS);
+        accumulate<T, kAhead>(s, v);
+    }
+    for (; i < p.vectors; i += THREADS) {
+        const uint4 v[1] = {__ldcg(body + i)};
+        accumulate<T, 1>(s, v);
+    }
+    if (threadIdx.x < p.head) accumulate_one(s, x[threadIdx.x]);
+    if (threadIdx.x < p.tail) accumulate_one(s, x[vocab - p.tail + threadIdx.x]);
+    return s;
+}
+
+// coefficient * (delta - p) for every logit of a row; `factor` = -coefficient / sum.
+template <typename T, int THREADS>
+__device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int target, const Exponent e, float factor, float coefficient, bool in_phase) {
+    const auto one = [&](int j) {
+        float value = exp2_fast(e(Vector<T>::load(x[j]))) * factor;
+        if (j == target) value += coefficient;
+        out[j] = Vector<T>::store(value);
+    };
+    if (!in_phase || e.extreme) {
+        for (int j = threadIdx.x; j < vocab; j += THREADS) one(j);
+        return;
+    }
+    constexpr int kCount = Vector<T>::kCount, kPairs = kCount / 2, kAhead = 4;
+    const Parts p = parts_of(x, vocab);
+    const uint4* body = reinterpret_cast<const uint4*>(x + p.head);
+    uint4* to = reinterpret_cast<uint4*>(out + p.head);
+    const int special = target >= p.head ? (target - p.head) / kCount : -1, place = (target - p.head) % kCount;
+    const Pair scale = pair(kLog2e, kLog2e), base = pair(-e.base, -e.base), by = pair(factor, factor);
+    const auto vector = [&](int i, const uint4& v) {
+        float2 f[kPairs];
+        Vector<T>::unpack(v, f);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            const float2 y = both(fma2(pair(f[k].x, f[k].y), scale, base));
+            f[k] = both(mul2(pair(exp2_fast(y.x), exp2_fast(y.y)), by));
+        }
+        if (i == special) {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                if (place == 2 * k) f[k].x += coefficient;
+                if (place == 2 * k + 1) f[k].y += coefficient;
+            }
+        }
+        __stcs(to + i, Vector<T>::pack(f));
+    };
+    int i = threadIdx.x;
+    for (; i + (kAhead - 1) * THREADS < p.vectors; i += kAhead * THREADS) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = __ldcs(body + i + k * THREADS);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) vector(i + k * THREADS, v[k]);
+    }
+    for (; i < p.vectors; i += THREADS) vector(i, __ldcs(body + i));
+    if (threadIdx.x < p.head) one(threadIdx.x);
+    if (threadIdx.x < p.tail) one(vocab - p.tail + threadIdx.x);
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void row_zero(T* out, int vocab) {
+    const Parts p = parts_of(out, vocab);
+    uint4* to = reinterpret_cast<uint4*>(out + p.head);
+    for (int i = threadIdx.x; i < p.vectors; i += THREADS) __stcs(to + i, make_uint4(0, 0, 0, 0));
+    if (threadIdx.x < p.head) out[threadIdx.x] = Vector<T>::store(0.f);
+    if (threadIdx.x < p.tail) out[vocab - p.tail + threadIdx.x] = Vector<T>::store(0.f);
+}
+
+__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
+
+template <typename T, Mode MODE, Loss LOSS, int THREADS>
+__global__ void __launch_bounds__(THREADS) token_rows_kernel(const __grid_constant__ Args a) {
     __shared__ Stat shared[32];
     __shared__ float shared_coefficient;
     __shared__ bool shared_last;
     const tk_token_rows& r = a.rows;
     const int64_t row = blockIdx.x, b = row / r.length, t = row % r.length;
     const T* x = static_cast<const T*>(r.logits) + b * r.stride_batch + t * r.stride_token;
-    T* out = static_cast<T*>(a.grad) + row * r.vocab;
+    T* out = static_cast<T*>(a.grad.data) + b * a.grad.stride_batch + t * a.grad.stride_token;
     const bool keep = counts(r, b, t);
-    const int64_t vocab = r.vocab;
-    float coefficient = 0.f, scale = 0.f;
+    const int vocab = static_cast<int>(r.vocab);
     Stat stat{kLowest, 0.f};
-    int64_t target = -1;
+    int target = -1;
     if (a.clear && row == 0 && threadIdx.x == 0) *a.clear = 0;
-    if (keep) target = target_of(r, b, t);
-    if (MODE != kGrad && keep) {
-        for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
-            const float value = to_float(x[j]);
-            if (value > stat.top) {
-                stat.sum *= exp2_fast((stat.top - value) * kLog2e);
-                stat.top = value;
-            }
-            stat.sum += exp2_fast((value - stat.top) * kLog2e);
-        }
-        stat = block_join(stat, shared);
+    if (keep) {
+        const int64_t wanted = target_of(r, b, t);
+        target = wanted >= 0 && wanted < vocab ? static_cast<int>(wanted) : -1;
     }
+    if (MODE != kGrad && keep) stat = block_join<THREADS>(row_stat<T, THREADS>(x, vocab), shared);
     if (MODE != kGrad && threadIdx.x == 0) {
         float logprob = 0.f;
-        if (keep) logprob = target >= 0 && target < vocab ? to_float(x[target]) - stat.top - logf(stat.sum) : __int_as_float(0x7fffffff);
+        if (keep) {
+            const Exponent e(stat.top);
+            const float value = target >= 0 ? Vector<T>::load(x[target]) : not_a_number();
+            logprob = e.extreme ? (value - stat.top) - logf(stat.sum) : (e(value) - log2f(stat.sum)) * kLn2;
+        }
         if (a.logprobs) a.logprobs[row] = logprob;
         if (a.stats) {
             a.stats[2 * row] = stat.top;
@@ -162,23 +394,18 @@ __global__ void __launch_bounds__(kThreads) token_rows_kernel(const __grid_const
     }
     if (MODE != kStats) {
         if (keep) {
-            scale = a.scale_at ? a.scale * *a.scale_at : a.scale;
+            float coefficient = a.grad.scale_at ? a.grad.scale * *a.grad.scale_at : a.grad.scale;
             if (LOSS == kPolicy) {
                 __syncthreads();
-                coefficient = shared_coefficient * scale;
+                coefficient *= shared_coefficient;
             } else {
-                coefficient = at(a.coefficients, b, t) * scale;
+                coefficient *= at(a.coefficients, b, t);
             }
             if (MODE == kGrad) stat = {a.stats[2 * row], a.stats[2 * row + 1]};
-            const bool known = target >= 0 && target < vocab;
-            const float factor = known ? -coefficient / stat.sum : __int_as_float(0x7fffffff);
-            for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
-                float value = exp2_fast((to_float(x[j]) - stat.top) * kLog2e) * factor;
-                if (j == target) value += coefficient;
-                out[j] = from_float<T>(value);
-            }
+            const float factor = target >= 0 ? -coefficient / stat.sum : not_a_number();
+            row_grad<T, THREADS>(out, x, vocab, target, Exponent(stat.top), factor, coefficient, a.in_phase);
         } else {
-            for (int64_t j = threadIdx.x; j < vocab; j += kThreads) out[j] = from_float<T>(0.f);
+            row_zero<T, THREADS>(out, vocab);
         }
     }
     if (MODE != kGrad && LOSS == kPolicy) {
@@ -190,13 +417,13 @@ __global__ void __launch_bounds__(kThreads) token_rows_kernel(const __grid_const
         }
         __syncthreads();
         if (shared_last) {
-            __shared__ double parts[kThreads];
+            __shared__ double parts[THREADS];
             double sum = 0.0;
             const int64_t rows = r.batch * r.length;
-            for (int64_t i = threadIdx.x; i < rows; i += kThreads) sum += __ldcg(a.terms + i);
+            for (int64_t i = threadIdx.x; i < rows; i += THREADS) sum += __ldcg(a.terms + i);
             parts[threadIdx.x] = sum;
             __syncthreads();
-            for (int step = kThreads / 2; step; step >>= 1) {
+            for (int step = THREADS / 2; step; step >>= 1) {
                 if (threadIdx.x < step) parts[threadIdx.x] += parts[threadIdx.x + step];
                 __syncthreads();
             }
@@ -285,13 +512,20 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int64_t pairs, in
     }
 }
 
+template <typename T, Mode MODE, Loss LOSS>
+void launch_type(const Args& a, unsigned grid, cudaStream_t stream) {
+    // A row of a few thousand logits gives 128 threads a handful of vectors each; more of them would idle in the join.
+    if (a.rows.vocab * sizeof(T) <= 128 * 16 * 8) token_rows_kernel<T, MODE, LOSS, 128><<<grid, 128, 0, stream>>>(a);
+    else token_rows_kernel<T, MODE, LOSS, 512><<<grid, 512, 0, stream>>>(a);
+}
+
 template <Mode MODE, Loss LOSS>
 int launch_rows(const Args& a, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(a.rows.batch * a.rows.length);
     switch (a.rows.dtype) {
-        case TK_F32: token_rows_kernel<float, MODE, LOSS><<<grid, kThreads, 0, stream>>>(a); break;
-        case TK_F16: token_rows_kernel<__half, MODE, LOSS><<<grid, kThreads, 0, stream>>>(a); break;
-        default: token_rows_kernel<__nv_bfloat16, MODE, LOSS><<<grid, kThreads, 0, stream>>>(a); break;
+        case TK_F32: launch_type<float, MODE, LOSS>(a, grid, stream); break;
+        case TK_F16: launch_type<__half, MODE, LOSS>(a, grid, stream); break;
+        default: launch_type<__nv_bfloat16, MODE, LOSS>(a, grid, stream); break;
     }
     count_launch();
     return check(cudaGetLastError(), "launching the token kernel");
@@ -299,7 +533,7 @@ int launch_rows(const Args& a, cudaStream_t stream) {
 
 int check_rows(const tk_token_rows* r, const char* who) {
     if (!r || !r->logits || !r->targets.data || r->batch < 1 || r->length < 1 || r->vocab < 1 || r->batch > 0x7fffffff / r->length
-        || r->vocab > 0x7fffffff || r->dtype < TK_F32 || r->dtype > TK_BF16 || (r->target_bytes != 4 && r->target_bytes != 8))
+        || r->vocab > 0x7ffffff0 || r->dtype < TK_F32 || r->dtype > TK_BF16 || (r->target_bytes != 4 && r->target_bytes != 8))
         return fail(TK_E_ARGUMENT, "trainkernel: invalid rows passed to %s", who);
     return 0;
 }
@@ -307,11 +541,13 @@ int check_rows(const tk_token_rows* r, const char* who) {
 Args arguments(const tk_token_rows* rows, const tk_token_grad* grad) {
     Args a{};
     a.rows = *rows;
-    a.scale = 1.f;
-    if (grad) {
-        a.grad = grad->data;
-        a.scale_at = grad->scale_at;
-        a.scale = grad->scale;
+    if (grad && grad->data) {
+        a.grad = *grad;
+        const int64_t bytes = rows->dtype == TK_F32 ? 4 : 2;
+        const auto apart = [&](int64_t x, int64_t y) { return (x - y) * bytes % 16 != 0; };
+        a.in_phase = (reinterpret_cast<uintptr_t>(rows->logits) - reinterpret_cast<uintptr_t>(grad->data)) % 16 == 0
+                     && (rows->batch == 1 || !apart(rows->stride_batch, grad->stride_batch))
+                     && (rows->length == 1 || !apart(rows->stride_token, grad->stride_token));
     }
     return a;
 }
@@ -383,7 +619,7 @@ extern "C" int tk_policy_loss(const tk_token_rows* rows, const tk_policy_terms* 
     policy_weights_kernel<<<1, 1024, 0, s>>>(*rows, terms->average, a.counter, a.weights);
     count_launch();
     if (int code = check(cudaGetLastError(), "launching the weight kernel")) return code;
-    return a.grad ? launch_rows<kBoth, kPolicy>(a, s) : launch_rows<kStats, kPolicy>(a, s);
+    return a.grad.data ? launch_rows<kBoth, kPolicy>(a, s) : launch_rows<kStats, kPolicy>(a, s);
 }
 
 extern "C" size_t tk_preference_workspace_bytes(int64_t batch, int64_t length) {

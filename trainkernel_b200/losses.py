@@ -15,7 +15,7 @@ strides as long as one row is contiguous, so the usual shifted slice `logits[:, 
 `targets` are int64 or int32.  `mask` is boolean, of the targets' shape; a row it excludes has
 log-probability 0 and gradient 0 whatever its logits hold, NaN included.  A counted target outside
 `[0, vocab)` reads nothing and gives NaN.  Log-probabilities, losses and sums are FP32; gradients have
-the logits' type.  Everything else that enters a loss is a constant: it must not require grad.
+the logits' type, and, for strided logits, their strides.  Everything else that enters a loss is a constant: it must not require grad.
 No counterpart in the reference, whose losses are means of squares (reference: benchmarks/train_loop.py:35-45).
 """
 from __future__ import annotations
@@ -155,6 +155,32 @@ def _fp32(shape, like: torch.Tensor) -> torch.Tensor:
     return torch.empty(shape, dtype=torch.float32, device=like.device)
 
 
+def _grad_like(logits: torch.Tensor) -> torch.Tensor:
+    """Room for the gradient.  It keeps the logits' row strides where that wastes little memory (a shifted slice of a
+    longer batch does), because rows that lie alike in memory are read and written 16 bytes at a time; otherwise dense."""
+    if logits.is_contiguous() and logits.storage_offset() * logits.element_size() % 16 == 0:
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
+    shape, strides = logits.shape, logits.stride()
+    order = sorted((s, n) for s, n in zip(strides, shape) if n > 1)
+    reach, apart = 1, True
+    for stride, size in order:
+        apart &= stride >= reach
+        reach += stride * (size - 1)
+    per = 16 // logits.element_size()
+    lead = logits.data_ptr() % 16 // logits.element_size()
+    if not apart or reach + per > 1.25 * logits.numel() + per:
+        return torch.empty(shape, dtype=logits.dtype, device=logits.device)
+    whole = torch.empty(lead + reach, dtype=logits.dtype, device=logits.device)
+    return whole.as_strided(shape, strides, lead)
+
+
+def _grad_struct(grad: torch.Tensor | None, scale: float, scale_at: torch.Tensor | None) -> TokenGrad:
+    if grad is None:
+        return TokenGrad(None, 0, 0, None, 1.0, 0)
+    strides = grad.stride()
+    return TokenGrad(grad.data_ptr(), strides[0] if grad.dim() == 3 else 0, strides[-2], _pointer(scale_at), scale, 0)
+
+
 def _logprobs_launch(logits, targets, mask, with_stats: bool):
     lib, device, stream = _place(logits)
     logprobs = _fp32(targets.shape, logits)
@@ -166,21 +192,21 @@ def _logprobs_launch(logits, targets, mask, with_stats: bool):
 def _logprobs_and_grad_launch(logits, targets, weights, mask, scale: float, scale_at):
     lib, device, stream = _place(logits)
     logprobs = _fp32(targets.shape, logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _grad_like(logits)
     operators.check(lib.tk_token_logprobs_and_grad(_row_struct(logits, targets, mask), TokenArray(*_array(weights, logits.dim())), logprobs.data_ptr(),
-                                                   TokenGrad(grad.data_ptr(), _pointer(scale_at), scale, 0), device, stream))
+                                                   _grad_struct(grad, scale, scale_at), device, stream))
     return logprobs, grad
 
 
 def _logits_grad_launch(logits, targets, mask, coefficients, stats, scale_at):
     lib, device, stream = _place(logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _grad_like(logits)
     if coefficients.dim() < targets.dim():
         array = TokenArray(coefficients.data_ptr(), coefficients.stride(0), 0)          # one per sequence
     else:
         array = TokenArray(*_array(coefficients, logits.dim()))
     operators.check(lib.tk_token_logits_grad(_row_struct(logits, targets, mask), array, stats.data_ptr(),
-                                             TokenGrad(grad.data_ptr(), _pointer(scale_at), 1.0, 0), device, stream))
+                                             _grad_struct(grad, 1.0, scale_at), device, stream))
     return grad
 
 
@@ -191,12 +217,12 @@ def _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_we
     loss, logprobs = _fp32((), logits), _fp32(shape, logits)
     stats = _fp32((*shape, 2), logits) if saved else None
     coefficients = _fp32(shape, logits) if saved else None
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+    out = _grad_like(logits) if grad else None
     rows = _row_struct(logits, targets, mask)
     workspace = torch.empty(lib.tk_policy_workspace_bytes(rows.batch, rows.length), dtype=torch.uint8, device=logits.device)
     terms = PolicyTerms(_array(old, rank), _array(advantages, rank), _array(ref, rank), low, high, kl_weight, average)
     operators.check(lib.tk_policy_loss(rows, terms, loss.data_ptr(), logprobs.data_ptr(), _pointer(stats), _pointer(coefficients),
-                                       TokenGrad(_pointer(out), _pointer(scale_at), scale, 0), workspace.data_ptr(), device, stream))
+                                       _grad_struct(out, scale, scale_at), workspace.data_ptr(), device, stream))
     return loss, logprobs, stats, coefficients, out
 
 
@@ -204,11 +230,11 @@ def _preference_launch(logits, targets, reference, mask, beta: float, smoothing:
     lib, device, stream = _place(logits)
     shape = targets.shape
     loss, sums, coefficients, stats = _fp32((), logits), _fp32(shape[:1], logits), _fp32(shape[:1], logits), _fp32((*shape, 2), logits)
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+    out = _grad_like(logits) if grad else None
     rows = _row_struct(logits, targets, mask)
     workspace = torch.empty(lib.tk_preference_workspace_bytes(rows.batch, rows.length), dtype=torch.uint8, device=logits.device)
     operators.check(lib.tk_preference_loss(rows, reference.data_ptr(), reference.stride(0), beta, smoothing, loss.data_ptr(), sums.data_ptr(),
-                                           stats.data_ptr(), coefficients.data_ptr(), TokenGrad(_pointer(out), _pointer(scale_at), scale, 0),
+                                           stats.data_ptr(), coefficients.data_ptr(), _grad_struct(out, scale, scale_at),
                                            workspace.data_ptr(), device, stream))
     return loss, sums, stats, coefficients, out
 

@@ -36,7 +36,7 @@ class TokenRows(ctypes.Structure):
 
 
 class TokenGrad(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("scale_at", ctypes.c_void_p), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    _fields_ = [("data", ctypes.c_void_p), ("stride_batch", ctypes.c_int64), ("stride_token", ctypes.c_int64), ("scale_at", ctypes.c_void_p), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
 class PolicyTerms(ctypes.Structure):

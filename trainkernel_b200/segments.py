@@ -215,7 +215,7 @@ class SegmentedProgram:
                         results = IMPLEMENTATIONS[step.op](*arguments)
                     results = (results,) if isinstance(results, torch.Tensor) else results
                     for op in step.results:
-                        values[op.output.buffer] = results[op.attrs["result"]]
+                        values[op.output.buffer] = results[op.attrs["result"]].contiguous()      # a gradient may have its logits' strides
                 for buffer in self._frees[index]:
                     values.pop(buffer, None)
             for slot, spec in enumerate(self.program.outputs):
