@@ -100,7 +100,7 @@ typedef struct {
 } tk_adamw_tensor;
 
 #define TK_ADAMW_BLOCK 256      /* elements that share one scale when moments are held in 8 bits */
-#define TK_ADAMW_COUNTERS 2048  /* copies of the step counter, one for each block that may be launched */
+#define TK_ADAMW_COUNTERS 4096  /* copies of the step counter, one for each block that may be launched */
 
 typedef struct {
     void* mean;                 /* FP32, or e4m3 codes */

@@ -70,14 +70,65 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// |value| <= 448 on one of the two e4m3 numbers around it: the larger one when the cut part exceeds `dither` / 2^16.
-// NaN stays NaN: every comparison with it is false, and floorf hands it on.
-__device__ __forceinline__ float round_e4m3(float value, uint32_t dither) {
-    float a = fabsf(value);
-    if (a > kE4m3Max) a = kE4m3Max;
-    const float normal = __uint_as_float((__float_as_uint(a) + (dither << 4)) & 0xfff00000u);
-    const float small = floorf(a * 512.f + static_cast<float>(dither) * (1.f / 65536.f)) * (1.f / 512.f);
-    return copysignf(a >= 0.015625f ? normal : small, value);
+// Two FP32 numbers in one 64-bit register: the paired instructions round each exactly as the single ones do.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float reciprocal(float x) {       // hardware approximation, 1 ulp
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float least(float a, float b) {   // NaN if either is
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Eight values on one of the two e4m3 numbers around each: the larger one when the cut part exceeds its 16 random bits.
+// From 2^-6 up an e4m3 number is an FP32 number without its last 20 bits, so adding the random bits above the last four
+// and cutting does it, whatever the sign (a value two units in the last place above 448 still ends on 448: the sum
+// carries only from sixteen on).  Below, they are multiples of 2^-9; that form is needed by few warps (a value 3e-5 of its
+// block's largest), so the warp asks once whether anybody needs it.  NaN takes it and stays NaN.  ROOT: a value
+// that stands for a number above zero (`above`) is not rounded to zero.
+template <bool ROOT>
+__device__ __forceinline__ void round8(float (&x)[8], const uint32_t (&random)[8], const float (&above)[8]) {
+    float smallest = kE4m3Max;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) smallest = least(smallest, fabsf(x[i]));
+    const bool any_small = __any_sync(~0u, !(smallest >= 0.015625f));
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t dither = ROOT ? random[i] >> 16 : random[i] & 0xffffu;
+        q[i] = __uint_as_float((__float_as_uint(x[i]) + (dither << 4)) & 0xfff00000u);
+    }
+    if (any_small) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t dither = ROOT ? random[i] >> 16 : random[i] & 0xffffu;
+            const float a = least(fabsf(x[i]), kE4m3Max), part = __uint_as_float(0x3f800000u | (dither << 7)) - 1.f;    // dither / 2^16
+            float whole = __fadd_rd(fmaf(a, 512.f, part), 8388608.f) - 8388608.f;                                       // rounded down: at most 9
+            if (ROOT && above[i] > 0.f && whole < 1.f) whole = 1.f;
+            if (!(a >= 0.015625f)) q[i] = copysignf(whole * (1.f / 512.f), x[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = q[i];
 }
 
 template <typename T> __device__ __forceinline__ void load8(float (&to)[8], const T* from, int64_t left, bool wide) {
@@ -128,14 +179,123 @@ __device__ __forceinline__ uint2 encode8(const float (&from)[8]) {
     return make_uint2(word[0], word[1]);
 }
 
-__device__ __forceinline__ float warp_max(float x) {
+// The largest of 32 non-negative numbers: their bit patterns have their order.
+__device__ __forceinline__ float warp_max(float x) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(x))); }
+
+struct Numbers {
+    Pair beta1, beta2, rest1, rest2, scale, spread, eps, pace;
+    uint32_t salt;
+};
+
+// One thread's eight elements: FULL when they, and the whole block of 256 around them, lie inside the tensor and on
+// 16-byte boundaries.  Otherwise lanes behind the tensor's end stay in the warp for the block maximum, with zeros.
+template <typename P, typename G, int BITS, bool FULL>
+__device__ __forceinline__ void update8(const tk_adamw_state& state, const Item& item, const Numbers& n, float decay, int64_t at, int64_t left) {
+    const int64_t flat = item.offset + at;
+    P* param = static_cast<P*>(item.param) + at;
+    const G* grad = static_cast<const G*>(item.grad) + at;
+    const bool wide_param = FULL || reinterpret_cast<uintptr_t>(item.param) % 16 == 0;
+    const bool wide_grad = FULL || reinterpret_cast<uintptr_t>(item.grad) % 16 == 0;
+    const int64_t inside = FULL ? 8 : left;
+    const bool in_block = FULL || left + (threadIdx.x % 32) * kPerThread > 0;
+    float p[8], g[8], m[8] = {}, v[8] = {};
+    float mean_scale = 0.f, root_scale = 0.f;
+    uint2 mean_codes = make_uint2(0, 0), root_codes = make_uint2(0, 0);
+    const int64_t block = flat / TK_ADAMW_BLOCK;
+    if (BITS == 8) {
+        if (in_block) {
+            mean_scale = state.mean_scale[block];
+            root_scale = state.root_scale[block];
+            mean_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(state.mean) + flat));
+            root_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(state.square) + flat));
+        }
+    } else if (FULL || left > 0) {
+        // the flat state is padded to whole blocks, so it is always read and written whole
+        load8<float>(m, static_cast<const float*>(state.mean) + flat, 8, true);
+        load8<float>(v, static_cast<const float*>(state.square) + flat, 8, true);
+    }
+    load8<P>(p, param, inside, wide_param);
+    load8<G>(g, grad, inside, wide_grad);
+    if (BITS == 8) {
+        decode8(m, mean_codes, mean_scale);
+        decode8(v, root_codes, root_scale);
+    }
+    float top_mean = 0.f, top_root = 0.f;
+    const Pair decays = pair(decay, decay);
 #pragma unroll
-    for (int step = 16; step; step >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, step));
-    return x;
+    for (int i = 0; i < 8; i += 2) {
+        const Pair gradient = mul2(pair(g[i], g[i + 1]), n.scale);
+        Pair square = pair(v[i], v[i + 1]);
+        if (BITS == 8) square = mul2(square, square);
+        float a, b, c, d;
+        const Pair kept1 = mul2(n.beta1, pair(m[i], m[i + 1])), new1 = mul2(n.rest1, gradient);
+        const Pair kept2 = mul2(n.beta2, square), new2 = mul2(mul2(n.rest2, gradient), gradient);
+        split(kept1, a, b);
+        split(new1, c, d);
+        m[i] = __fadd_rn(a, c);                              // single additions: paired ones are fused with the products
+        m[i + 1] = __fadd_rn(b, d);
+        split(kept2, a, b);
+        split(new2, c, d);
+        v[i] = __fadd_rn(a, c);
+        v[i + 1] = __fadd_rn(b, d);
+        const Pair mean = pair(m[i], m[i + 1]);
+        a = sqrtf(v[i]);
+        b = sqrtf(v[i + 1]);
+        split(fma2(pair(a, b), n.spread, n.eps), c, d);
+        // p decay - pace m / (sqrt(v) spread + eps)
+        const Pair change = mul2(mul2(n.pace, mean), pair(reciprocal(c), reciprocal(d)));
+        split(fma2(pair(p[i], p[i + 1]), decays, change ^ 0x8000000080000000ull), p[i], p[i + 1]);
+        if (BITS == 8) {
+            v[i] = a;
+            v[i + 1] = b;
+            if (FULL || i < inside) top_mean = fmaxf(top_mean, fabsf(m[i])), top_root = fmaxf(top_root, a);
+            if (FULL || i + 1 < inside) top_mean = fmaxf(top_mean, fabsf(m[i + 1])), top_root = fmaxf(top_root, b);
+        }
+    }
+    store8<P>(param, p, inside, wide_param);
+    if (BITS == 8) {
+        top_mean = warp_max(top_mean);
+        top_root = warp_max(top_root);
+        const float mean_factor = top_mean >= kSmallest ? __fmul_rn(__frcp_rn(top_mean), kE4m3Max) : 0.f;
+        const float root_factor = top_root >= kSmallest ? __fmul_rn(__frcp_rn(top_root), kE4m3Max) : 0.f;
+        const Pair mean_factors = pair(mean_factor, mean_factor), root_factors = pair(root_factor, root_factor);
+        uint32_t random[8];
+        float root[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) random[i] = mix(static_cast<uint32_t>(flat) ^ n.salt ^ i);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            split(mul2(pair(m[i], m[i + 1]), mean_factors), m[i], m[i + 1]);
+            split(mul2(pair(v[i], v[i + 1]), root_factors), root[i], root[i + 1]);
+        }
+        round8<false>(m, random, v);
+        round8<true>(root, random, v);
+        if (!FULL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i >= inside) m[i] = root[i] = 0.f;
+        }
+        if (in_block) {
+            __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(state.mean) + flat), encode8(m));
+            __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(state.square) + flat), encode8(root));
+            if (threadIdx.x % 32 == 0) {
+                state.mean_scale[block] = top_mean >= kSmallest ? __fmul_rn(top_mean, 1.f / kE4m3Max) : 0.f;
+                state.root_scale[block] = top_root >= kSmallest ? __fmul_rn(top_root, 1.f / kE4m3Max) : 0.f;
+            }
+        }
+    } else if (FULL || left > 0) {
+        if (!FULL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i >= inside) m[i] = v[i] = 0.f;
+        }
+        store8<float>(static_cast<float*>(state.mean) + flat, m, 8, true);
+        store8<float>(static_cast<float*>(state.square) + flat, v, 8, true);
+    }
 }
 
 template <typename P, typename G, int BITS, int CAPACITY>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Args<CAPACITY> a) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Args<CAPACITY> a) {
     const float scale = a.scale_at ? *a.scale_at : 1.f;
     if (!(fabsf(scale) <= 3.402823466e38f)) return;                    // not finite: this step does not happen
     const int64_t step = a.state.steps[blockIdx.x] + 1;
@@ -144,11 +304,20 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     const float left1 = -expm1f(static_cast<float>(static_cast<double>(step) * a.log_beta1));
     const float left2 = -expm1f(static_cast<float>(static_cast<double>(step) * a.log_beta2));
     const float pace = lr / left1, spread = 1.f / sqrtf(left2);
-    const uint32_t salt = mix(static_cast<uint32_t>(step) + a.seed * 0x9e3779b9u);
+    Numbers n;
+    n.beta1 = pair(a.beta1, a.beta1);
+    n.beta2 = pair(a.beta2, a.beta2);
+    n.rest1 = pair(a.one_minus_beta1, a.one_minus_beta1);
+    n.rest2 = pair(a.one_minus_beta2, a.one_minus_beta2);
+    n.scale = pair(scale, scale);
+    n.spread = pair(spread, spread);
+    n.eps = pair(a.eps, a.eps);
+    n.pace = pair(pace, pace);
+    n.salt = mix(static_cast<uint32_t>(step) + a.seed * 0x9e3779b9u);
 
-    // Each block takes a contiguous run of chunks, so it searches for its first tensor once and walks on from there.
-    const int begin = static_cast<int>(static_cast<int64_t>(a.chunks) * blockIdx.x / gridDim.x);
-    const int end = static_cast<int>(static_cast<int64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
+    // Chunks are dealt out one by one, so that blocks that run together touch neighbouring memory (contiguous runs per
+    // block took 135 us where this takes 113 us: 33.5M elements, 8-bit moments, FP32 gradients).
+    const int begin = blockIdx.x;
     int low = 0, high = a.count - 1;
     while (low < high) {
         const int middle = (low + high + 1) / 2;
@@ -156,87 +325,16 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         else high = middle - 1;
     }
     int which = low;
-    for (int chunk = begin; chunk < end; ++chunk) {
+    for (int chunk = begin; chunk < a.chunks; chunk += gridDim.x) {
         while (which + 1 < a.count && a.items[which + 1].first_chunk <= chunk) ++which;
         const Item& item = a.items[which];
         const int64_t at = static_cast<int64_t>(chunk - item.first_chunk) * kChunk + threadIdx.x * kPerThread;
         const int64_t left = item.count - at;
-        const int64_t flat = item.offset + at;
-        P* param = static_cast<P*>(item.param) + at;
-        const G* grad = static_cast<const G*>(item.grad) + at;
-        const bool wide_param = reinterpret_cast<uintptr_t>(item.param) % 16 == 0, wide_grad = reinterpret_cast<uintptr_t>(item.grad) % 16 == 0;
-        float p[8], g[8], m[8] = {}, v[8] = {};
-        // Lanes behind the tensor's end stay in the warp for the block maximum; their values are zeros.
-        const bool inside = left > 0;
-        uint2 mean_codes = make_uint2(0, 0), root_codes = make_uint2(0, 0);
-        float mean_scale = 0.f, root_scale = 0.f;
-        const int64_t block = flat / TK_ADAMW_BLOCK;
-        const bool block_inside = item.count - (at - (threadIdx.x % 32) * kPerThread) > 0;
-        if (BITS == 8) {
-            if (block_inside) {
-                mean_scale = a.state.mean_scale[block];
-                root_scale = a.state.root_scale[block];
-                mean_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.state.mean) + flat));
-                root_codes = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.state.square) + flat));
-            }
-        }
-        load8<P>(p, param, left, wide_param);
-        load8<G>(g, grad, left, wide_grad);
-        if (BITS == 8) {
-            decode8(m, mean_codes, mean_scale);
-            decode8(v, root_codes, root_scale);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
-        } else {
-            // the flat state is padded to whole blocks, so it is always read and written whole
-            if (inside) {
-                load8<float>(m, static_cast<const float*>(a.state.mean) + flat, 8, true);
-                load8<float>(v, static_cast<const float*>(a.state.square) + flat, 8, true);
-            }
-        }
         const float decay = 1.f - lr * item.weight_decay;
-        float top_mean = 0.f, top_root = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float gradient = i < left ? __fmul_rn(g[i], scale) : 0.f;
-            m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.one_minus_beta1, gradient));
-            v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(__fmul_rn(a.one_minus_beta2, gradient), gradient));
-            const float root = sqrtf(v[i]);
-            p[i] = p[i] * decay - pace * m[i] / (root * spread + a.eps);
-            if (BITS == 8) {
-                v[i] = root;
-                if (i < left) {
-                    top_mean = fmaxf(top_mean, fabsf(m[i]));
-                    top_root = fmaxf(top_root, root);
-                }
-            }
-        }
-        store8<P>(param, p, left, wide_param);
-        if (BITS == 8) {
-            top_mean = warp_max(top_mean);
-            top_root = warp_max(top_root);
-            if (block_inside) {
-                const float mean_factor = top_mean >= kSmallest ? __fmul_rn(__frcp_rn(top_mean), kE4m3Max) : 0.f;
-                const float root_factor = top_root >= kSmallest ? __fmul_rn(__frcp_rn(top_root), kE4m3Max) : 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t random = mix(static_cast<uint32_t>(flat + i) ^ salt);
-                    const float root = v[i];
-                    m[i] = i < left ? round_e4m3(__fmul_rn(m[i], mean_factor), random & 0xffff) : 0.f;
-                    v[i] = i < left ? round_e4m3(__fmul_rn(root, root_factor), random >> 16) : 0.f;
-                    if (i < left && root > 0.f && v[i] < 1.f / 512.f) v[i] = 1.f / 512.f;
-                }
-                __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.state.mean) + flat), encode8(m));
-                __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.state.square) + flat), encode8(v));
-                if (threadIdx.x % 32 == 0) {
-                    a.state.mean_scale[block] = top_mean >= kSmallest ? __fmul_rn(top_mean, 1.f / kE4m3Max) : 0.f;
-                    a.state.root_scale[block] = top_root >= kSmallest ? __fmul_rn(top_root, 1.f / kE4m3Max) : 0.f;
-                }
-            }
-        } else if (inside) {
-            store8<float>(static_cast<float*>(a.state.mean) + flat, m, 8, true);
-            store8<float>(static_cast<float*>(a.state.square) + flat, v, 8, true);
-        }
+        const bool whole = item.count - static_cast<int64_t>(chunk - item.first_chunk) * kChunk >= kChunk
+                           && (reinterpret_cast<uintptr_t>(item.param) | reinterpret_cast<uintptr_t>(item.grad)) % 16 == 0;
+        if (whole) update8<P, G, BITS, true>(a.state, item, n, decay, at, left);
+        else update8<P, G, BITS, false>(a.state, item, n, decay, at, left);
     }
     // Only this block reads the counters it advances, so no block can see another's new value.
     if (a.last)
@@ -249,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 }
 
 template <typename P, typename G, int BITS, int CAPACITY>
-int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, cudaStream_t stream) {
     Args<CAPACITY> a;
     a.state = *state;
     a.lr_at = o->lr_at;
@@ -272,7 +370,9 @@ int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* stat
         if (chunks > 0x7fffffff) return fail(TK_E_ARGUMENT, "trainkernel: too many elements in one tk_adamw_update");
     }
     a.chunks = static_cast<int32_t>(chunks);
-    int64_t grid = static_cast<int64_t>(sms) * 8;
+    // Several waves, so that the hardware evens out what blocks take (33.5M elements, 32-bit moments: 170 us with one wave
+    // of 592 blocks, 164 with two, 157 with three, 148 with six).
+    int64_t grid = chunks;
     if (grid > TK_ADAMW_COUNTERS) grid = TK_ADAMW_COUNTERS;
     if (grid > chunks) grid = chunks;
     if (grid < 1) grid = 1;
@@ -282,27 +382,27 @@ int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* stat
 }
 
 template <typename P, typename G, int BITS>
-int launch_all(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+int launch_all(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, cudaStream_t stream) {
     while (count > kMany) {
-        if (int code = launch<P, G, BITS, kMany>(tensors, kMany, state, o, 0, sms, stream)) return code;
+        if (int code = launch<P, G, BITS, kMany>(tensors, kMany, state, o, 0, stream)) return code;
         tensors += kMany;
         count -= kMany;
     }
-    return count > kFew ? launch<P, G, BITS, kMany>(tensors, count, state, o, last, sms, stream)
-                        : launch<P, G, BITS, kFew>(tensors, count, state, o, last, sms, stream);
+    return count > kFew ? launch<P, G, BITS, kMany>(tensors, count, state, o, last, stream)
+                        : launch<P, G, BITS, kFew>(tensors, count, state, o, last, stream);
 }
 
 template <typename P, typename G>
-int by_bits(const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
-    return o->bits == 8 ? launch_all<P, G, 8>(t, n, s, o, last, sms, stream) : launch_all<P, G, 32>(t, n, s, o, last, sms, stream);
+int by_bits(const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, cudaStream_t stream) {
+    return o->bits == 8 ? launch_all<P, G, 8>(t, n, s, o, last, stream) : launch_all<P, G, 32>(t, n, s, o, last, stream);
 }
 
 template <typename P>
-int by_grad(int dtype, const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int sms, cudaStream_t stream) {
+int by_grad(int dtype, const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, cudaStream_t stream) {
     switch (dtype) {
-        case TK_F32: return by_bits<P, float>(t, n, s, o, last, sms, stream);
-        case TK_F16: return by_bits<P, __half>(t, n, s, o, last, sms, stream);
-        default: return by_bits<P, __nv_bfloat16>(t, n, s, o, last, sms, stream);
+        case TK_F32: return by_bits<P, float>(t, n, s, o, last, stream);
+        case TK_F16: return by_bits<P, __half>(t, n, s, o, last, stream);
+        default: return by_bits<P, __nv_bfloat16>(t, n, s, o, last, stream);
     }
 }
 
@@ -321,12 +421,10 @@ extern "C" int tk_adamw_update(const tk_adamw_tensor* tensors, int count, int pa
             return fail(TK_E_ARGUMENT, "trainkernel: invalid tensor %d passed to tk_adamw_update", i);
     DeviceScope scope(device);
     if (scope.status) return scope.status;
-    const int sms = tk_ops::sm_count(device);
-    if (sms < 1) return fail(TK_E_ARGUMENT, "trainkernel: device %d cannot be asked for its multiprocessors", device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (param_dtype) {
-        case TK_F32: return by_grad<float>(grad_dtype, tensors, count, state, options, last, sms, s);
-        case TK_F16: return by_grad<__half>(grad_dtype, tensors, count, state, options, last, sms, s);
-        default: return by_grad<__nv_bfloat16>(grad_dtype, tensors, count, state, options, last, sms, s);
+        case TK_F32: return by_grad<float>(grad_dtype, tensors, count, state, options, last, s);
+        case TK_F16: return by_grad<__half>(grad_dtype, tensors, count, state, options, last, s);
+        default: return by_grad<__nv_bfloat16>(grad_dtype, tensors, count, state, options, last, s);
     }
 }

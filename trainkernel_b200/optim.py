@@ -19,7 +19,7 @@ from . import operators
 from .operators import AdamWOptions, AdamWTensor
 
 BLOCK = 256                 # elements that share one scale when moments are held in 8 bits
-_COUNTERS = 2048            # copies of the step counter (TK_ADAMW_COUNTERS)
+_COUNTERS = 4096            # copies of the step counter (TK_ADAMW_COUNTERS)
 
 
 class AdamWState:
