@@ -285,6 +285,31 @@ def test_tiny_and_vanishing_moments_stay_numbers():
     assert all(bool(torch.isfinite(x).all()) for x in state.moments(0))
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_short_and_long_way_to_a_launch_agree(bits, monkeypatch):
+    from trainkernel_b200 import operators
+    sizes = [300, 0, 5, 4096]
+    results = []
+    for long_way in (False, True):
+        if long_way:
+            monkeypatch.setattr(operators, "fast", None)
+        p, g = tensors(sizes, F32, 1.0, 50), tensors(sizes, BF16, 0.1, 51)
+        optimizer = tk.AdamW(weight_decay=(0.0, 0.1, 0.2, 0.3), state_bits=bits, seed=9)
+        state = optimizer.init(p)
+        if not long_way:
+            assert operators.fast.adamw_update(p, g, state.sizes, state.offsets, 0.0, state._struct_at, state._tensors, bits, 0.0, (0.9, 0.9), 1e-8, 0, None)
+            p, g = tensors(sizes, F32, 1.0, 50), tensors(sizes, BF16, 0.1, 51)
+            state = optimizer.init(p)
+        for _ in range(2):
+            before = [x._version for x in (*p, *state.tensors())]
+            optimizer.update(p, g, state, grad_scale=torch.full((), 0.5, device="cuda"))
+            assert all(x._version > v for x, v in zip((*p, *state.tensors()), before))
+        results.append([*p, *state.tensors()])
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # -- refusals ------------------------------------------------------------------------------------------------
 
 def test_refusals_of_numbers():

@@ -466,14 +466,61 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(logp, again[0]) and torch.equal(grad, again[1])
 
 
+@gpu
+def test_short_and_long_way_to_a_launch_agree(monkeypatch):
+    from trainkernel_b200 import operators
+    logits, targets, mask = make((2, 3), 50, F32, 39)
+    old, one = torch.zeros((2, 3), device="cuda"), torch.ones((2, 1), device="cuda")
+    tk.token_logprobs(logits, targets)
+    for answer in (operators.fast.token_logprobs(logits, targets, None), operators.fast.token_logprobs_and_grad(logits, targets, old, None, 1.0),
+                   operators.fast.policy_loss(logits, targets, old, one, None, None, (0.2, 0.2), 0.0, "tokens", 1.0),
+                   operators.fast.preference_loss(logits, targets, one[:, 0], None, 0.1, 0.0, None)):
+        assert answer is not None                              # an ordinary call does go the short way
+    assert operators.fast.token_logprobs(logits.requires_grad_(), targets, None) is None
+    results = []
+    for long_way in (False, True):
+        if long_way:
+            monkeypatch.setattr(operators, "fast", None)
+        taken = []
+        for shape, vocab, dtype, layout, masked in (((4, 6), 1000, BF16, "dense", True), ((4, 6), 777, F32, "shift", False), ((2, 8), 40, F16, "pitch", True), ((12,), 129, F32, "dense", False)):
+            logits, targets, mask = make(shape, vocab, dtype, 40, layout=layout, masked=masked)
+            old, adv, reference = noise(shape, 0.3, 41) - 6, noise((*shape[:-1], 1), 1.0, 42) if len(shape) == 2 else noise(shape, 1.0, 42), noise(shape[:1], 1.0, 43)
+            taken += [tk.token_logprobs(logits, targets, mask=mask), *tk.token_logprobs_and_grad(logits, targets, old, mask=mask, grad_scale=2)]
+            taken += [*tk.policy_loss(logits, targets, old, adv, mask=mask), *tk.policy_loss_and_grad(logits, targets, old, adv, mask=mask, ref_logprobs=old, kl_weight=1)]
+            if len(shape) == 2:
+                taken += [*tk.preference_loss(logits, targets, reference, mask=mask), *tk.preference_loss_and_grad(logits, targets, reference, mask=mask, grad_scale=0.5)]
+        results.append(taken)
+    for a, b in zip(*results):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a, b)
+
+
+@gpu
+def test_transformed_constants_are_refused():
+    logits, targets, _ = make((3,), 20, F32, 44)
+    with pytest.raises(ValueError, match="detach"):
+        torch.func.grad(lambda a: tk.policy_loss_and_grad(logits, targets, torch.zeros(3, device="cuda"), a)[0])(torch.ones(3, device="cuda"))
+
+
 # -- refusals (no GPU) ---------------------------------------------------------------------------------------
 
-def _cpu(shape=(2, 3), vocab=5):
-    return torch.randn(*shape, vocab), torch.zeros(shape, dtype=torch.int64), torch.zeros(shape)
+def _cpu(shape=(2, 3), vocab=5, device="cpu"):
+    return torch.randn(*shape, vocab, device=device), torch.zeros(shape, dtype=torch.int64, device=device), torch.zeros(shape, device=device)
 
 
-def test_refusals_of_rows():
-    logits, targets, old = _cpu()
+ON = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+
+
+def on_device(device):
+    """On the GPU a first good call makes the compiled host path the one that is asked first."""
+    if device == "cuda":
+        logits, targets, _ = _cpu(device="cuda")
+        tk.token_logprobs(logits, targets)
+    return device
+
+
+@ON
+def test_refusals_of_rows(device):
+    logits, targets, old = _cpu(device=on_device(device))
     bad = [
         (lambda: tk.token_logprobs(logits.double(), targets), "float32, float16 or bfloat16"),
         (lambda: tk.token_logprobs(logits, targets.float()), "int64 or int32"),
@@ -483,14 +530,14 @@ def test_refusals_of_rows():
         (lambda: tk.token_logprobs(logits[:, :0], targets[:, :0]), "empty"),
         (lambda: tk.token_logprobs(logits[..., :0], targets), "empty"),
         (lambda: tk.token_logprobs(logits.transpose(1, 2).contiguous().transpose(1, 2), targets), "contiguous"),
-        (lambda: tk.token_logprobs(logits, targets, mask=torch.ones(2, 3)), "boolean"),
-        (lambda: tk.token_logprobs(logits, targets, mask=torch.ones(2, 1, dtype=torch.bool)), "shape"),
+        (lambda: tk.token_logprobs(logits, targets, mask=torch.ones(2, 3, device=device)), "boolean"),
+        (lambda: tk.token_logprobs(logits, targets, mask=torch.ones(2, 1, dtype=torch.bool, device=device)), "shape"),
         (lambda: tk.token_logprobs(logits, targets.to("meta")), "one device"),
         (lambda: tk.token_logprobs_and_grad(logits, targets, old.double()), "float32"),
-        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(7)), "broadcast"),
+        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(7, device=device)), "broadcast"),
         (lambda: tk.token_logprobs_and_grad(logits, targets, old.requires_grad_()), "detach"),
-        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(3), grad_scale="big"), "grad_scale"),
-        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(3), grad_scale=torch.ones(2)), "grad_scale"),
+        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(3, device=device), grad_scale="big"), "grad_scale"),
+        (lambda: tk.token_logprobs_and_grad(logits, targets, torch.zeros(3, device=device), grad_scale=torch.ones(2, device=device)), "grad_scale"),
     ]
     for call, message in bad:
         with pytest.raises(ValueError, match=message):
@@ -501,8 +548,9 @@ def test_refusals_of_rows():
         tk.token_logprobs_and_grad(logits, targets, 1.0)
 
 
-def test_refusals_of_the_losses():
-    logits, targets, old = _cpu()
+@ON
+def test_refusals_of_the_losses(device):
+    logits, targets, old = _cpu(device=on_device(device))
     bad = [
         (lambda: tk.policy_loss(logits, targets, old, old, kl_weight=0.1), "needs ref_logprobs"),
         (lambda: tk.policy_loss(logits, targets, old, old, kl_weight=-1.0, ref_logprobs=old), "kl_weight"),
@@ -511,12 +559,12 @@ def test_refusals_of_the_losses():
         (lambda: tk.policy_loss(logits, targets, old, old, clip=(1.5, 0.2)), "clip below"),
         (lambda: tk.policy_loss(logits, targets, old, old, average="rows"), "average"),
         (lambda: tk.policy_loss(logits, targets, old, old.half()), "float32"),
-        (lambda: tk.policy_loss_and_grad(logits, targets, old, torch.zeros(3, 2)), "broadcast"),
-        (lambda: tk.preference_loss(logits[:1], targets[:1], torch.zeros(1)), "even number"),
-        (lambda: tk.preference_loss(logits[0], targets[0], torch.zeros(3)), "sequences, length, vocab"),
+        (lambda: tk.policy_loss_and_grad(logits, targets, old, torch.zeros(3, 2, device=device)), "broadcast"),
+        (lambda: tk.preference_loss(logits[:1], targets[:1], torch.zeros(1, device=device)), "even number"),
+        (lambda: tk.preference_loss(logits[0], targets[0], torch.zeros(3, device=device)), "sequences, length, vocab"),
         (lambda: tk.preference_loss(logits, targets, old), "one summed"),
-        (lambda: tk.preference_loss(logits, targets, torch.zeros(2), beta=-0.1), "beta"),
-        (lambda: tk.preference_loss(logits, targets, torch.zeros(2), label_smoothing=1.5), "label_smoothing"),
+        (lambda: tk.preference_loss(logits, targets, torch.zeros(2, device=device), beta=-0.1), "beta"),
+        (lambda: tk.preference_loss(logits, targets, torch.zeros(2, device=device), label_smoothing=1.5), "label_smoothing"),
     ]
     for call, message in bad:
         with pytest.raises(ValueError, match=message):

@@ -413,10 +413,11 @@ def _differentiable(function: type[torch.autograd.Function], *args):
     return function.apply(*args)
 
 
-def _is_plain(logits: torch.Tensor) -> bool:
-    """Real tensors, no tracing, no transform, no history to record: the launch can be made directly."""
-    return (type(logits) in (torch.Tensor, torch.nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(logits)
-            and not torch._C._len_torch_dispatch_stack())
+def _is_plain(*tensors: torch.Tensor | None) -> bool:
+    """Real tensors, no tracing, no transform: the launch can be made directly (when there is no history to record)."""
+    wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+    return not torch._C._len_torch_dispatch_stack() and all(
+        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) and not wrapped(t) for t in tensors)
 
 
 def _records(who: str, logits: torch.Tensor) -> bool:
@@ -436,8 +437,10 @@ def _records(who: str, logits: torch.Tensor) -> bool:
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, mask: torch.Tensor | None = None) -> torch.Tensor:
     """`log_softmax(logits)[targets]` in FP32, one value per row; differentiable in the logits."""
+    if operators.fast is not None and (done := operators.fast.token_logprobs(logits, targets, mask)) is not None:
+        return done
     _check_rows("token_logprobs", logits, targets, mask)
-    if _is_plain(logits) and not _records("token_logprobs", logits):
+    if _is_plain(logits, targets, mask) and not _records("token_logprobs", logits):
         return _logprobs_launch(logits, targets, mask, False)[0]
     return _differentiable(_TokenLogprobs, logits, targets, mask)[0]
 
@@ -449,11 +452,13 @@ def token_logprobs_and_grad(logits: torch.Tensor, targets: torch.Tensor, weights
     With `weights = -1 / count` this is the cross entropy and its gradient in one pass over the logits.
     `weights` is FP32 and broadcasts to the targets' shape.
     """
+    if operators.fast is not None and (done := operators.fast.token_logprobs_and_grad(logits, targets, weights, mask, grad_scale)) is not None:
+        return done
     who = "token_logprobs_and_grad"
     _check_rows(who, logits, targets, mask)
     weights = _check_constant(who, "weights", weights, targets.shape, logits.device)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits):
+    if _is_plain(logits, targets, weights, mask):
         return _logprobs_and_grad_launch(logits, targets, weights, mask, scale, scale_at)
     _no_tensor_scale(who, scale_at)
     return _call.token_logprobs_and_grad(logits, targets, weights, mask, scale)
@@ -469,9 +474,12 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
     `average="tokens"` averages over all counted tokens; `"sequences"` over the tokens of each sequence and then over
     all `batch` sequences (one without counted tokens contributes 0).  With nothing counted the loss is 0.
     """
+    if operators.fast is not None and (done := operators.fast.policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip,
+                                                                          kl_weight, average, None)) is not None:
+        return done
     who = "policy_loss"
     old, advantages, ref, low, high, kl_weight, which = _check_policy(who, logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip, kl_weight, average)
-    if _is_plain(logits) and not _records(who, logits):
+    if _is_plain(logits, targets, old, advantages, ref, mask) and not _records(who, logits):
         return _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_weight, which, saved=False, grad=False)[:2]
     return _differentiable(_PolicyLoss, logits, targets, old, advantages, ref, mask, low, high, kl_weight, which)[:2]
 
@@ -481,10 +489,13 @@ def policy_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, old_logpro
                          kl_weight: float = 0.0, average: str = "tokens",
                          grad_scale: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """`(loss, logprobs, grad)`: `policy_loss` with the gradient of `grad_scale * loss` in the logits, in one pass."""
+    if operators.fast is not None and grad_scale is not None and (
+            done := operators.fast.policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip, kl_weight, average, grad_scale)) is not None:
+        return done
     who = "policy_loss_and_grad"
     old, advantages, ref, low, high, kl_weight, which = _check_policy(who, logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip, kl_weight, average)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits):
+    if _is_plain(logits, targets, old, advantages, ref, mask):
         loss, logprobs, _, _, grad = _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_weight, which, saved=False, grad=True,
                                                     scale=scale, scale_at=scale_at)
         return loss, logprobs, grad
@@ -509,9 +520,12 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: torc
     `h = (sums[i] - reference[i]) - (sums[j] - reference[j])` a pair's loss is
     `-(1 - label_smoothing) log sigmoid(beta h) - label_smoothing log sigmoid(-beta h)`, and the loss is their mean.
     """
+    if operators.fast is not None and (
+            done := operators.fast.preference_loss(logits, targets, reference, mask, beta, label_smoothing, None)) is not None:
+        return done
     who = "preference_loss"
     reference, beta, label_smoothing = _check_preference(who, logits, targets, reference, mask, beta, label_smoothing)
-    if _is_plain(logits) and not _records(who, logits):
+    if _is_plain(logits, targets, reference, mask) and not _records(who, logits):
         return _preference_launch(logits, targets, reference, mask, beta, label_smoothing, grad=False)[:2]
     return _differentiable(_PreferenceLoss, logits, targets, reference, mask, beta, label_smoothing)[:2]
 
@@ -520,10 +534,13 @@ def preference_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, refere
                              beta: float = 0.1, label_smoothing: float = 0.0,
                              grad_scale: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """`(loss, sums, grad)`: `preference_loss` with the gradient of `grad_scale * loss` in the logits."""
+    if operators.fast is not None and grad_scale is not None and (
+            done := operators.fast.preference_loss(logits, targets, reference, mask, beta, label_smoothing, grad_scale)) is not None:
+        return done
     who = "preference_loss_and_grad"
     reference, beta, label_smoothing = _check_preference(who, logits, targets, reference, mask, beta, label_smoothing)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits):
+    if _is_plain(logits, targets, reference, mask):
         loss, sums, _, _, grad = _preference_launch(logits, targets, reference, mask, beta, label_smoothing, grad=True, scale=scale, scale_at=scale_at)
         return loss, sums, grad
     _no_tensor_scale(who, scale_at)

@@ -8,7 +8,9 @@ tensors that are not on an sm_100 device raise.  No counterpart in the reference
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import subprocess
+import sysconfig
 import threading
 from pathlib import Path
 
@@ -21,8 +23,11 @@ SOURCES = ("tk_token_rows.cu", "tk_adamw.cu", "tk_ops_host.cpp")
 HEADERS = ("tk_ops_host.h",)
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
-_lock = threading.Lock()
+HOST_PATH = runtime.PACKAGE_DIR / "_ops_host.so"
+
+_lock = threading.RLock()
 _library: ctypes.CDLL | None = None
+_host = None
 
 
 class TokenArray(ctypes.Structure):
@@ -76,6 +81,40 @@ def build_library(force: bool = False) -> Path:
     return LIBRARY_PATH
 
 
+def build_host(force: bool = False) -> Path:
+    """Compile `csrc/tk_ops_host_path.cpp`, the short way from a Python call to a launch, against PyTorch's headers."""
+    source = runtime.CSRC_DIR / "tk_ops_host_path.cpp"
+    library_path = build_library()
+    watched = (source, runtime.INCLUDE_DIR / "trainkernel_ops.h")
+    if not force and HOST_PATH.exists() and HOST_PATH.stat().st_mtime >= max(p.stat().st_mtime for p in watched):
+        return HOST_PATH
+    cuda = runtime._cuda_home()
+    if cuda is None:
+        raise RuntimeError("trainkernel: CUDA toolkit headers are required to build the operators' host path")
+    torch_dir = Path(torch.__file__).resolve().parent
+    include = [runtime.INCLUDE_DIR, torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", Path(cuda) / "include",
+               sysconfig.get_paths()["include"]]
+    command = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *(f"-I{path}" for path in include), "-o", str(HOST_PATH), str(source), f"-L{torch_dir / 'lib'}", f"-L{library_path.parent}",
+               "-ltrainkernel_ops", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    done = subprocess.run(command, capture_output=True, text=True)
+    if done.returncode != 0:
+        raise RuntimeError(f"trainkernel: building the operators' host path failed:\n{done.stderr[-4000:]}")
+    return HOST_PATH
+
+
+def host():
+    """The compiled host path (its calls return None for anything out of the ordinary)."""
+    global _host
+    with _lock:
+        if _host is None:
+            library()                           # resident first: the host path links against it
+            spec = importlib.util.spec_from_file_location("_ops_host", build_host())
+            _host = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(_host)
+        return _host
+
+
 def library() -> ctypes.CDLL:
     """The loaded operator library with argument types declared; built on first use if missing."""
     global _library
@@ -107,16 +146,21 @@ def check(code: int) -> None:
 
 
 _usable: dict[int, bool] = {}
+fast = None             # the host path, once a device has been found usable
 
 
 def require_device(device: torch.device) -> int:
     """The ordinal of an sm_100 CUDA device; raises for anything else, as `compile_program` does."""
     if device.type != "cuda":
         raise RuntimeError("trainkernel: CUDA sm_100a GPU required; this operator has no CPU form")
+    global fast
     index = device.index if device.index is not None else torch.cuda.current_device()
     if index not in _usable:
         capability = torch.cuda.get_device_capability(index)
         _usable[index] = capability[0] == 10
+        if _usable[index]:
+            host().allow_device(index)
+            fast = host()
     if not _usable[index]:
         raise RuntimeError("trainkernel: an sm_100 (B200-class) GPU is required")
     return index

@@ -57,6 +57,8 @@ class AdamWState:
         self._second = second
         self._struct = operators.AdamWState(self.exp_avg.data_ptr(), second.data_ptr(), *(None if s is None else s.data_ptr() for s in scales),
                                             self._counters.data_ptr())
+        self._struct_at = ctypes.addressof(self._struct)
+        self._tensors = self.tensors()
 
     @property
     def step(self) -> torch.Tensor:
@@ -183,6 +185,10 @@ class AdamW:
         device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
         not happen: parameters, moments and step count stay as they are.
         """
+        if operators.fast is not None and state.bits == self.state_bits and operators.fast.adamw_update(
+                params, grads, state.sizes, state.offsets, self.weight_decay, state._struct_at, state._tensors, self.state_bits, self.lr, self.betas,
+                self.eps, self.seed, grad_scale) is not None:
+            return
         leaves, gradients = _leaves(params, "params"), _leaves(grads, "grads")
         device = state.device
         if state.bits != self.state_bits:
