@@ -140,7 +140,7 @@ SHAPES = [
     ((1, 3), 511, BF16, "dense"), ((2, 5), 513, F32, "shift"), ((4, 7), 1000, BF16, "shift"), ((3, 4), 4099, F16, "shift"), ((2, 3), 4097, BF16, "pitch"),
     ((2, 9), 6007, F32, "pitch"), ((2, 3), 32000, BF16, "swapped"), ((1, 2), 50257, BF16, "shift"), ((2, 2), 50257, F32, "shift"), ((3,), 65537, F16, "dense"),
     ((2,), 128256, BF16, "dense"), ((1, 2), 151937, F32, "dense"), ((1,), 262144, BF16, "dense"), ((1,), 300001, BF16, "pitch"), ((257, 3), 129, BF16, "dense"),
-    ((700,), 24, F32, "dense"), ((31, 40), 520, F16, "shift"),
+    ((700,), 24, F32, "dense"), ((31, 40), 520, F16, "shift"), ((40, 30), 20011, BF16, "shift"), ((500,), 33000, F32, "dense"), ((9, 100), 70001, F16, "shift"),
 ]
 IDS = [f"{'x'.join(map(str, s))}x{v}-{str(d).split('.')[1]}-{lay}" for s, v, d, lay in SHAPES]
 
@@ -179,14 +179,15 @@ def test_policy_loss_and_gradient(shape, vocab, dtype, layout, masked, average, 
     # a log-probability is off by d (bound above); the ratio and the KL slope by d + 8 u relative; slope also cancels between its two parts
     x = clean(logits, mask).double()
     d = float(U * (4 * (x.amax(-1) - x.amin(-1)).max() + vocab / 256 + 40))
-    weight = 1.0 / (1 if mask is None else max(1, int(mask.sum())))
     parts = (advantages.abs().double().expand(shape) * 1.5 + kl * 4).max()
     assert abs(float(loss) - float(want)) <= float(parts) * (d + 16 * U) * 1.5 + 4 * U
     scaled = slope * 2.0
     assert_slope_grad(grad, clean(logits, mask), targets, scaled, mask, float(parts) * (d + 16 * U), average, shape)
     only, logp2 = tk.policy_loss(logits, targets, old, advantages, ref_logprobs=ref, mask=mask, clip=clip, kl_weight=kl, average=average)
-    assert torch.equal(only, loss) and torch.equal(logp2, logp)
-    assert weight > 0
+    # the form without a gradient may split a row between other threads and so add its terms in another order: it keeps to
+    # the same bounds, not to the same bits
+    assert_logprobs(logp2, clean(logits, mask), targets, mask)
+    assert abs(float(only) - float(want)) <= float(parts) * (d + 16 * U) * 1.5 + 4 * U
 
 
 def assert_slope_grad(got, logits, targets, scaled, mask, error, average, shape):

@@ -157,8 +157,9 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, Vector<T>::top(v[i]));
     const Exponent e(top);
-    if (top > s.top) s = join(s, {top, 0.f});
     if (!e.extreme) {
+        s.sum *= exp2_fast(scaled(s.top) - e.base);        // as in join; 0 while nothing was added
+        s.top = top;
         const Pair scale = pair(kLog2e, kLog2e), base = pair(-e.base, -e.base);
         Pair sum = pair(0.f, 0.f);
 #pragma unroll
@@ -174,6 +175,7 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
         const float2 total = both(sum);
         s.sum += total.x + total.y;
     } else {
+        s = join(s, {top, 0.f});
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float2 f[kPairs];
@@ -192,6 +194,8 @@ __device__ __forceinline__ void accumulate_one(Stat& s, T value) {
 }
 
 enum Mode { kStats, kGrad, kBoth };            // log-probabilities / gradient from saved stats / both
+constexpr int kFirstRows = 2048;               // more rows than blocks run at once
+
 enum Loss { kWeights, kPolicy };               // where kBoth takes the coefficient from, and what kStats adds
 
 struct Args {
@@ -224,36 +228,43 @@ __device__ __forceinline__ float at(const tk_token_array& a, int64_t b, int64_t 
     return static_cast<const float*>(a.data)[b * a.stride_batch + t * a.stride_token];
 }
 
+// The statistics of 32 lanes, in every lane: the largest top first, then the sums relative to it.
+__device__ __forceinline__ Stat warp_join(Stat mine) {
+    float top = mine.top;
+#pragma unroll
+    for (int step = 16; step; step >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, step));
+    float sum = join(mine, {top, 0.f}).sum;
+#pragma unroll
+    for (int step = 16; step; step >>= 1) sum += __shfl_xor_sync(~0u, sum, step);
+    return {top, sum};
+}
+
 template <int THREADS>
 __device__ Stat block_join(Stat mine, Stat* shared) {
-#pragma unroll
-    for (int step = 16; step; step >>= 1)
-        mine = join(mine, {__shfl_xor_sync(~0u, mine.top, step), __shfl_xor_sync(~0u, mine.sum, step)});
+    mine = warp_join(mine);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (lane == 0) shared[warp] = mine;
     __syncthreads();
-    mine = lane < THREADS / 32 ? shared[lane] : Stat{kLowest, 0.f};
-#pragma unroll
-    for (int step = 16; step; step >>= 1)
-        mine = join(mine, {__shfl_xor_sync(~0u, mine.top, step), __shfl_xor_sync(~0u, mine.sum, step)});
-    return mine;
+    return warp_join(lane < THREADS / 32 ? shared[lane] : Stat{kLowest, 0.f});
 }
 
 // The loss of one token and its slope in the log-probability.
-__device__ __forceinline__ void policy_token(const tk_policy_terms& p, int64_t b, int64_t t, float logprob, float* term, float* slope) {
-    const float advantage = at(p.advantages, b, t);
-    const float ratio = expf(logprob - at(p.old_logprobs, b, t));
+__device__ __forceinline__ void policy_token(const tk_policy_terms& p, float old_logprob, float advantage, float ref_logprob, float logprob,
+                                             float* term, float* slope) {
+    const float ratio = expf(logprob - old_logprob);
     const float free = ratio * advantage;
     const float bound = fminf(fmaxf(ratio, 1.f - p.clip_low), 1.f + p.clip_high) * advantage;
     const bool clipped = free > bound;                    // false for NaN: it then stays in the result
     *term = clipped ? -bound : -free;
     *slope = clipped ? 0.f : -free;
     if (p.ref_logprobs.data) {
-        const float away = at(p.ref_logprobs, b, t) - logprob, grown = expm1f(away);
+        const float away = ref_logprob - logprob, grown = expm1f(away);
         *term += p.kl_weight * (grown - away);
         *slope -= p.kl_weight * grown;
     }
 }
+
+__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
 
 // A row's parts: elements before the first 16-byte boundary, whole vectors, elements behind the last.
 struct Parts {
@@ -267,17 +278,47 @@ __device__ __forceinline__ Parts parts_of(const T* x, int vocab) {
     return {head, (vocab - head) / kCount, (vocab - head) % kCount};
 }
 
+// Loads that ask L2 to keep a line (it is read again soon) or to let go of it.
+__device__ __forceinline__ uint4 load_hint(const uint4* p, unsigned long long policy) {
+    uint4 v;
+    asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
+    return v;
+}
+__device__ __forceinline__ unsigned long long keep_policy() {
+    unsigned long long policy;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+
+constexpr int kAhead = 4;                      // vectors a thread has in flight
+
+// Statistics of a row.  The first `kept` vectors (a multiple of kAhead * THREADS, or the whole row) also go to shared
+// memory, where the thread that read them finds them again.
 template <typename T, int THREADS>
-__device__ __forceinline__ Stat row_stat(const T* x, int vocab) {
-    constexpr int kAhead = 4;                  // vectors a thread has in flight
+__device__ __forceinline__ Stat row_stat(const T* x, int vocab, uint4* kept_at, int kept, bool again) {
     const Parts p = parts_of(x, vocab);
     const uint4* body = reinterpret_cast<const uint4*>(x + p.head);
     Stat s{kLowest, 0.f};
     int i = threadIdx.x;
+    const int first = min(kept, p.vectors);
+    for (; i + (kAhead - 1) * THREADS < first; i += kAhead * THREADS) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = __ldcs(body + i + k * THREADS);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) kept_at[i + k * THREADS] = v[k];
+        accumulate<T, kAhead>(s, v);
+    }
+    for (; i < first; i += THREADS) {
+        const uint4 v[1] = {__ldcs(body + i)};
+        kept_at[i] = v[0];
+        accumulate<T, 1>(s, v);
+    }
+    const unsigned long long policy = keep_policy();
     for (; i + (kAhead - 1) * THREADS < p.vectors; i += kAhead * THREADS) {
         uint4 v[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) v[k] = __ldcg(body + i + k * THREADS);
+        for (int k = 0; k < kAhead; ++k) v[k] = again ? load_hint(body + i + k * THREADS, policy) : __ldcg(body + i + k * THREADS);
         accumulate<T, kAhead>(s, v);
     }
     for (; i < p.vectors; i += THREADS) {
@@ -291,7 +332,8 @@ __device__ __forceinline__ Stat row_stat(const T* x, int vocab) {
 
 // coefficient * (delta - p) for every logit of a row; `factor` = -coefficient / sum.
 template <typename T, int THREADS>
-__device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int target, const Exponent e, float factor, float coefficient, bool in_phase) {
+__device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int target, const Exponent e, float factor, float coefficient, bool in_phase,
+                                         const uint4* kept_at, int kept) {
     const auto one = [&](int j) {
         float value = exp2_fast(e(Vector<T>::load(x[j]))) * factor;
         if (j == target) value += coefficient;
@@ -301,7 +343,7 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int targ
         for (int j = threadIdx.x; j < vocab; j += THREADS) one(j);
         return;
     }
-    constexpr int kCount = Vector<T>::kCount, kPairs = kCount / 2, kAhead = 4;
+    constexpr int kCount = Vector<T>::kCount, kPairs = kCount / 2;
     const Parts p = parts_of(x, vocab);
     const uint4* body = reinterpret_cast<const uint4*>(x + p.head);
     uint4* to = reinterpret_cast<uint4*>(out + p.head);
@@ -324,15 +366,17 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int targ
         }
         __stcs(to + i, Vector<T>::pack(f));
     };
-    int i = threadIdx.x;
-    for (; i + (kAhead - 1) * THREADS < p.vectors; i += kAhead * THREADS) {
+    // From the row's end, which was read last and is near, to the part kept in shared memory.
+    const int first = min(kept, p.vectors), left = (p.vectors - first) % (kAhead * THREADS);
+    for (int i = p.vectors - kAhead * THREADS + threadIdx.x; i >= first + left; i -= kAhead * THREADS) {
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) v[k] = __ldcs(body + i + k * THREADS);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) vector(i + k * THREADS, v[k]);
     }
-    for (; i < p.vectors; i += THREADS) vector(i, __ldcs(body + i));
+    for (int i = first + threadIdx.x; i < first + left; i += THREADS) vector(i, __ldcs(body + i));
+    for (int i = threadIdx.x; i < first; i += THREADS) vector(i, kept_at[i]);
     if (threadIdx.x < p.head) one(threadIdx.x);
     if (threadIdx.x < p.tail) one(vocab - p.tail + threadIdx.x);
 }
@@ -346,10 +390,35 @@ __device__ __forceinline__ void row_zero(T* out, int vocab) {
     if (threadIdx.x < p.tail) out[vocab - p.tail + threadIdx.x] = Vector<T>::store(0.f);
 }
 
-__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
+// Kernels that follow another one of the same call are launched while it still runs and wait here for its results.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-template <typename T, Mode MODE, Loss LOSS, int THREADS>
-__global__ void __launch_bounds__(THREADS) token_rows_kernel(const __grid_constant__ Args a) {
+__device__ __forceinline__ float row_logprob(Stat stat, float value) {
+    const Exponent e(stat.top);
+    return e.extreme ? (value - stat.top) - logf(stat.sum) : (e(value) - log2f(stat.sum)) * kLn2;
+}
+
+// The sum of all rows' terms in an order that does not depend on which block forms it.
+template <int THREADS>
+__device__ __forceinline__ void sum_terms(const float* terms, int64_t rows, float* loss) {
+    __shared__ double parts[32];
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < rows; i += THREADS) sum += __ldcg(terms + i);
+#pragma unroll
+    for (int step = 16; step; step >>= 1) sum += __shfl_xor_sync(~0u, sum, step);
+    if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = 0.0;
+        for (int i = 0; i < THREADS / 32; ++i) sum += parts[i];
+        *loss = static_cast<float>(sum);
+    }
+}
+
+template <typename T, Mode MODE, Loss LOSS, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __grid_constant__ Args a, const int kept) {
+    extern __shared__ uint4 kept_at[];
     __shared__ Stat shared[32];
     __shared__ float shared_coefficient;
     __shared__ bool shared_last;
@@ -366,14 +435,26 @@ __global__ void __launch_bounds__(THREADS) token_rows_kernel(const __grid_consta
         const int64_t wanted = target_of(r, b, t);
         target = wanted >= 0 && wanted < vocab ? static_cast<int>(wanted) : -1;
     }
-    if (MODE != kGrad && keep) stat = block_join<THREADS>(row_stat<T, THREADS>(x, vocab), shared);
-    if (MODE != kGrad && threadIdx.x == 0) {
-        float logprob = 0.f;
-        if (keep) {
-            const Exponent e(stat.top);
-            const float value = target >= 0 ? Vector<T>::load(x[target]) : not_a_number();
-            logprob = e.extreme ? (value - stat.top) - logf(stat.sum) : (e(value) - log2f(stat.sum)) * kLn2;
+    // What the row's result needs besides its statistics is asked for before them, so that it has arrived behind them.
+    float value = not_a_number(), old_logprob = 0.f, advantage = 0.f, ref_logprob = 0.f, weight = 0.f;
+    if (MODE != kGrad && keep && threadIdx.x == 0) {
+        if (target >= 0) value = Vector<T>::load(x[target]);
+        if (LOSS == kPolicy) {
+            old_logprob = at(a.policy.old_logprobs, b, t);
+            advantage = at(a.policy.advantages, b, t);
+            if (a.policy.ref_logprobs.data) ref_logprob = at(a.policy.ref_logprobs, b, t);
+            // The first blocks start beside the kernel that computes the weights and ask for theirs behind the statistics.
+            if (row >= kFirstRows) {
+                wait_for_previous();
+                weight = a.weights[b];
+            }
         }
+    }
+    if (MODE == kGrad) wait_for_previous();
+    if (MODE != kStats && LOSS != kPolicy && keep) weight = at(a.coefficients, b, t);
+    if (MODE != kGrad && keep) stat = block_join<THREADS>(row_stat<T, THREADS>(x, vocab, kept_at, kept, MODE == kBoth), shared);
+    if (MODE != kGrad && threadIdx.x == 0) {
+        const float logprob = keep ? row_logprob(stat, value) : 0.f;
         if (a.logprobs) a.logprobs[row] = logprob;
         if (a.stats) {
             a.stats[2 * row] = stat.top;
@@ -381,9 +462,10 @@ __global__ void __launch_bounds__(THREADS) token_rows_kernel(const __grid_consta
         }
         if (LOSS == kPolicy) {
             float term = 0.f, slope = 0.f;
+            if (row < kFirstRows) wait_for_previous();
             if (keep) {
-                policy_token(a.policy, b, t, logprob, &term, &slope);
-                const float weight = a.weights[b];
+                if (row < kFirstRows) weight = a.weights[b];
+                policy_token(a.policy, old_logprob, advantage, ref_logprob, logprob, &term, &slope);
                 term *= weight;
                 slope *= weight;
             }
@@ -399,42 +481,36 @@ __global__ void __launch_bounds__(THREADS) token_rows_kernel(const __grid_consta
                 __syncthreads();
                 coefficient *= shared_coefficient;
             } else {
-                coefficient *= at(a.coefficients, b, t);
+                coefficient *= weight;
             }
             if (MODE == kGrad) stat = {a.stats[2 * row], a.stats[2 * row + 1]};
             const float factor = target >= 0 ? -coefficient / stat.sum : not_a_number();
-            row_grad<T, THREADS>(out, x, vocab, target, Exponent(stat.top), factor, coefficient, a.in_phase);
+            row_grad<T, THREADS>(out, x, vocab, target, Exponent(stat.top), factor, coefficient, a.in_phase, kept_at, kept);
         } else {
             row_zero<T, THREADS>(out, vocab);
         }
     }
-    if (MODE != kGrad && LOSS == kPolicy) {
-        // The block that finishes last adds the terms of all rows, in an order that does not depend on who that is.
+    if (MODE != kGrad && LOSS == kPolicy && a.counter) {
+        // The block that finishes last adds the terms of all rows.
         if (threadIdx.x == 0) {
             __threadfence();
             shared_last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
             __threadfence();
         }
         __syncthreads();
-        if (shared_last) {
-            __shared__ double parts[THREADS];
-            double sum = 0.0;
-            const int64_t rows = r.batch * r.length;
-            for (int64_t i = threadIdx.x; i < rows; i += THREADS) sum += __ldcg(a.terms + i);
-            parts[threadIdx.x] = sum;
-            __syncthreads();
-            for (int step = THREADS / 2; step; step >>= 1) {
-                if (threadIdx.x < step) parts[threadIdx.x] += parts[threadIdx.x + step];
-                __syncthreads();
-            }
-            if (threadIdx.x == 0) *a.loss = static_cast<float>(parts[0]);
-        }
+        if (shared_last) sum_terms<THREADS>(a.terms, r.batch * r.length, a.loss);
     }
+}
+
+__global__ void __launch_bounds__(1024) policy_sum_kernel(const float* terms, int64_t rows, float* loss) {
+    wait_for_previous();
+    sum_terms<1024>(terms, rows, loss);
 }
 
 // What one counted token of every sequence weighs in the loss, from the mask alone, and the finish counter at zero.
 __global__ void __launch_bounds__(1024) policy_weights_kernel(tk_token_rows r, int average, unsigned* counter, float* weights) {
     __shared__ long long shared_total;
+    let_next_start();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         shared_total = 0;
@@ -463,6 +539,7 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int64_t pairs, in
                                                                float* coefficients, unsigned* counter, float* terms, float* loss) {
     __shared__ double parts[2][8];
     __shared__ bool shared_last;
+    wait_for_previous();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t pair = blockIdx.x;
 #pragma unroll
@@ -512,23 +589,52 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int64_t pairs, in
     }
 }
 
+// `early`: the kernel may start while the previous one of this call runs; it waits for it itself.
+template <typename... A>
+int launch(void (*kernel)(A...), int64_t grid, int threads, size_t shared, bool early, cudaStream_t stream, A... arguments) {
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(grid));
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = early ? 1 : 0;
+    count_launch();
+    return check(cudaLaunchKernelEx(&config, kernel, arguments...), "launching a token kernel");
+}
+
+constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
+
+// How many threads share a row, and so how many rows are in flight.  More, smaller blocks hide one another's joins:
+// 16384 x 8000 BF16 logits with gradient take 126 us with 16 blocks of 128 threads on an SM, 134 with 12, 149 with 8; rows
+// of 62 KB take 205 us (8000 of them) with 5 blocks of 256 threads, 234 with 4 and 314 with 2 of 640.  For long rows the
+// second read has to find the row in L2, and few rows may be in flight: 4096 rows of 250 KB take 388 us with 2 blocks of
+// 640 threads that keep the first 80 KB of their row in shared memory, 417 without keeping it, 444 with 3 of 512.
 template <typename T, Mode MODE, Loss LOSS>
-void launch_type(const Args& a, unsigned grid, cudaStream_t stream) {
-    // A row of a few thousand logits gives 128 threads a handful of vectors each; more of them would idle in the join.
-    if (a.rows.vocab * sizeof(T) <= 128 * 16 * 8) token_rows_kernel<T, MODE, LOSS, 128><<<grid, 128, 0, stream>>>(a);
-    else token_rows_kernel<T, MODE, LOSS, 512><<<grid, 512, 0, stream>>>(a);
+int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
+    const int64_t bytes = a.rows.vocab * static_cast<int64_t>(sizeof(T)), grid = a.rows.batch * a.rows.length;
+    if (bytes <= 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 128, 16>, grid, 128, 0, early, stream, a, 0);
+    if (MODE != kBoth) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3>, grid, 512, 0, early, stream, a, 0);
+    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 5>, grid, 256, 0, early, stream, a, 0);
+    auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2>;
+    static std::atomic<bool> sized[64];
+    if (device >= 64 || !sized[device].load(std::memory_order_relaxed)) {
+        if (int code = check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptVectors * 16), "sizing shared memory")) return code;
+        if (device < 64) sized[device].store(true, std::memory_order_relaxed);
+    }
+    return launch(kernel, grid, 640, kKeptVectors * 16, early, stream, a, kKeptVectors);
 }
 
 template <Mode MODE, Loss LOSS>
-int launch_rows(const Args& a, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(a.rows.batch * a.rows.length);
+int launch_rows(const Args& a, int device, bool early, cudaStream_t stream) {
     switch (a.rows.dtype) {
-        case TK_F32: launch_type<float, MODE, LOSS>(a, grid, stream); break;
-        case TK_F16: launch_type<__half, MODE, LOSS>(a, grid, stream); break;
-        default: launch_type<__nv_bfloat16, MODE, LOSS>(a, grid, stream); break;
+        case TK_F32: return launch_type<float, MODE, LOSS>(a, device, early, stream);
+        case TK_F16: return launch_type<__half, MODE, LOSS>(a, device, early, stream);
+        default: return launch_type<__nv_bfloat16, MODE, LOSS>(a, device, early, stream);
     }
-    count_launch();
-    return check(cudaGetLastError(), "launching the token kernel");
 }
 
 int check_rows(const tk_token_rows* r, const char* who) {
@@ -563,7 +669,7 @@ extern "C" int tk_token_logprobs(const tk_token_rows* rows, float* logprobs, flo
     Args a = arguments(rows, nullptr);
     a.logprobs = logprobs;
     a.stats = stats;
-    return launch_rows<kStats, kWeights>(a, static_cast<cudaStream_t>(stream));
+    return launch_rows<kStats, kWeights>(a, device, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tk_token_logprobs_and_grad(const tk_token_rows* rows, const tk_token_array* weights, float* logprobs,
@@ -576,7 +682,7 @@ extern "C" int tk_token_logprobs_and_grad(const tk_token_rows* rows, const tk_to
     Args a = arguments(rows, grad);
     a.coefficients = *weights;
     a.logprobs = logprobs;
-    return launch_rows<kBoth, kWeights>(a, static_cast<cudaStream_t>(stream));
+    return launch_rows<kBoth, kWeights>(a, device, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tk_token_logits_grad(const tk_token_rows* rows, const tk_token_array* coefficients, const float* stats,
@@ -589,7 +695,7 @@ extern "C" int tk_token_logits_grad(const tk_token_rows* rows, const tk_token_ar
     Args a = arguments(rows, grad);
     a.coefficients = *coefficients;
     a.stats = const_cast<float*>(stats);
-    return launch_rows<kGrad, kWeights>(a, static_cast<cudaStream_t>(stream));
+    return launch_rows<kGrad, kWeights>(a, device, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t tk_policy_workspace_bytes(int64_t batch, int64_t length) {
@@ -616,10 +722,15 @@ extern "C" int tk_policy_loss(const tk_token_rows* rows, const tk_policy_terms* 
     a.weights = reinterpret_cast<float*>(at + 16);
     a.terms = reinterpret_cast<float*>(at + 16 + padded(4 * static_cast<size_t>(rows->batch)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    policy_weights_kernel<<<1, 1024, 0, s>>>(*rows, terms->average, a.counter, a.weights);
-    count_launch();
-    if (int code = check(cudaGetLastError(), "launching the weight kernel")) return code;
-    return a.grad.data ? launch_rows<kBoth, kPolicy>(a, s) : launch_rows<kStats, kPolicy>(a, s);
+    if (int code = launch(policy_weights_kernel, 1, 1024, 0, false, s, *rows, static_cast<int>(terms->average), a.counter, a.weights)) return code;
+    // A few rows: their last block adds the terms, which saves a launch.  Many rows: every block would wait for its
+    // answer from the counter, and a launch of its own is cheaper.
+    const int64_t count = rows->batch * rows->length;
+    const bool apart = count > 1024;
+    if (apart) a.counter = nullptr;
+    if (int code = a.grad.data ? launch_rows<kBoth, kPolicy>(a, device, true, s) : launch_rows<kStats, kPolicy>(a, device, true, s)) return code;
+    if (!apart) return 0;
+    return launch(policy_sum_kernel, 1, 1024, 0, true, s, static_cast<const float*>(a.terms), count, loss);
 }
 
 extern "C" size_t tk_preference_workspace_bytes(int64_t batch, int64_t length) {
@@ -644,15 +755,13 @@ extern "C" int tk_preference_loss(const tk_token_rows* rows, const float* refere
     a.logprobs = logprobs;
     a.stats = stats;
     a.clear = counter;
-    if (int code = launch_rows<kStats, kWeights>(a, s)) return code;
+    if (int code = launch_rows<kStats, kWeights>(a, device, false, s)) return code;
     const int64_t pairs = rows->batch / 2;
-    preference_pairs_kernel<<<static_cast<unsigned>(pairs), 256, 0, s>>>(pairs, rows->length, logprobs, reference, reference_stride, beta,
-                                                                         label_smoothing, sums, coefficients, counter, terms, loss);
-    count_launch();
-    if (int code = check(cudaGetLastError(), "launching the pair kernel")) return code;
+    if (int code = launch(preference_pairs_kernel, pairs, 256, 0, true, s, pairs, rows->length, static_cast<const float*>(logprobs), reference,
+                          reference_stride, beta, label_smoothing, sums, coefficients, counter, terms, loss)) return code;
     if (!grad || !grad->data) return 0;
     Args g = arguments(rows, grad);
     g.stats = stats;
     g.coefficients = {coefficients, 1, 0};
-    return launch_rows<kGrad, kWeights>(g, s);
+    return launch_rows<kGrad, kWeights>(g, device, true, s);
 }
