@@ -313,7 +313,7 @@ def test_short_and_long_way_to_a_launch_agree(bits, monkeypatch):
 # -- refusals ------------------------------------------------------------------------------------------------
 
 def test_refusals_of_numbers():
-    bad = [dict(lr=-1.0), dict(lr=float("nan")), dict(lr=torch.ones(1)), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(betas=(0.9,)), dict(eps=0.0),
+    bad = [dict(lr=-1.0), dict(lr=float("nan")), dict(lr=torch.ones(1)), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(betas=(0.9,)), dict(eps=0.0), dict(eps=1e-40),
            dict(weight_decay=-0.1), dict(weight_decay=[0.1, "x"]), dict(state_bits=16), dict(seed=-1), dict(seed=2 ** 32)]
     for arguments in bad:
         with pytest.raises(ValueError, match="trainkernel: AdamW"):
@@ -325,6 +325,52 @@ def test_parameters_on_the_host_are_refused():
         tk.AdamW().init([torch.zeros(3)])
     with pytest.raises(TypeError, match="tensors only"):
         tk.AdamW().init([1.0])
+
+
+@gpu
+def test_init_inside_a_capture_is_refused():
+    p = [torch.zeros(4, device="cuda")]
+    tk.AdamW().init(p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="clear the moments"):
+            tk.AdamW().init(p)
+        p[0].add_(1.0)
+
+
+@gpu
+@pytest.mark.parametrize("betas", [(0.0, 0.0), (0.9, 0.0), (0.0, 0.999)])
+def test_betas_of_zero(betas):
+    p, g = tensors([700], F32, 1.0, 60), tensors([700], F32, 0.1, 61)
+    g[0][:5] = 0
+    optimizer = tk.AdamW(lr=1e-2, betas=betas, weight_decay=0.0)
+    state = optimizer.init(p)
+    for t in (1, 2):
+        before, old = p[0].double(), [x.double() for x in state.moments(0)]
+        optimizer.update(p, g, state)
+        want = exact(before, g[0].double(), *old, t, 1e-2, betas, 1e-8, 0.0)
+        check_param(p[0], want[0], want[3])
+
+
+@gpu
+def test_an_update_leaves_gradients_and_follows_the_current_stream():
+    p, g = tensors([5000, 3], F32, 1.0, 62), tensors([5000, 3], F32, 0.1, 63)
+    kept = [x.clone() for x in g]
+    optimizer = tk.AdamW()
+    state, other = optimizer.init(p), [x.clone() for x in p]
+    twin = optimizer.init(other)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            optimizer.update(p, g, state)
+    for _ in range(3):
+        optimizer.update(other, g, twin)
+    torch.cuda.synchronize()
+    for a, b in zip([*p, *state.tensors()], [*other, *twin.tensors()]):
+        assert torch.equal(a, b)
+    assert all(torch.equal(a, b) for a, b in zip(g, kept))
 
 
 @gpu

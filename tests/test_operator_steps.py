@@ -109,6 +109,14 @@ def test_capture_refuses_what_the_operators_refuse():
         tk.compile_training(lambda p: (p.sum(), p, p), (x,), optimizer=tk.AdamW())
 
 
+def test_sharded_steps_refuse_the_operators():
+    from trainkernel_b200 import dp
+    example = cases.data("cpu")
+    for form in (dp.ShardedTrainingStep, dp.FusedShardedTrainingStep):
+        with pytest.raises(ValueError, match="cannot call the token operators"):
+            form(cases.policy_step, example)
+
+
 def test_masks_are_accepted_as_inputs_and_nothing_else_is_done_with_them():
     with pytest.raises(ValueError, match="unsupported"):
         tk.capture(lambda m: m & m, (torch.ones(3, dtype=torch.bool),))
@@ -200,6 +208,9 @@ def test_late_commit_and_optimizer_refusals():
     runner = tk.compile(lambda w, ids: (w * 2.0, tk.token_logprobs(w, ids)), (w, ids), inplace_outputs={0: 0})
     doubled, logp = runner(w, ids)
     assert doubled.data_ptr() == w.data_ptr() and torch.equal(w, kept * 2.0) and torch.equal(logp, tk.token_logprobs(kept, ids))
+    for use in (lambda: runner.runner.allocate(w, ids), lambda: runner.runner.run_into(w, ids, buffers=None), lambda: runner.runner.module):
+        with pytest.raises(ValueError, match="several launches"):
+            use()
     example = cases.data("cuda")
     step = tk.compile_training(cases.policy_gradients, example, optimizer=tk.AdamW())
     with pytest.raises(ValueError, match="shape, stride"):

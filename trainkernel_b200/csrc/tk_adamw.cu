@@ -88,7 +88,8 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-__device__ __forceinline__ float reciprocal(float x) {       // hardware approximation, 1 ulp
+// Hardware approximation, 1 ulp; the divisor is at least eps, which the entry point keeps among the normal numbers.
+__device__ __forceinline__ float reciprocal(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
@@ -413,7 +414,7 @@ extern "C" int tk_adamw_update(const tk_adamw_tensor* tensors, int count, int pa
     if (!tensors || count < 1 || !state || !options || !state->mean || !state->square || !state->steps || param_dtype < TK_F32
         || param_dtype > TK_BF16 || grad_dtype < TK_F32 || grad_dtype > TK_BF16 || (options->bits != 8 && options->bits != 32)
         || (options->bits == 8 && (!state->mean_scale || !state->root_scale)) || !(options->beta1 >= 0 && options->beta1 < 1)
-        || !(options->beta2 >= 0 && options->beta2 < 1))
+        || !(options->beta2 >= 0 && options->beta2 < 1) || !(options->eps >= 1e-30))
         return fail(TK_E_ARGUMENT, "trainkernel: invalid argument to tk_adamw_update");
     for (int i = 0; i < count; ++i)
         if (tensors[i].count < 0 || tensors[i].offset < 0 || tensors[i].offset % TK_ADAMW_BLOCK

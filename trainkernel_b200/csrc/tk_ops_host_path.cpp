@@ -245,7 +245,8 @@ PyObject* adamw_update(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (n < 1 || PySequence_Fast_GET_SIZE(grads) != n || PyTuple_GET_SIZE(sizes) != n || (PyTuple_CheckExact(decay) && PyTuple_GET_SIZE(decay) != n)) Py_RETURN_NONE;
         tk_adamw_options options{};
         double bits = 0, seed = 0;
-        if (!number(args[8], &options.lr) || !PyTuple_CheckExact(args[9]) || PyTuple_GET_SIZE(args[9]) != 2 || !number(PyTuple_GET_ITEM(args[9], 0), &options.beta1)
+        const bool lr_given = number(args[8], &options.lr);
+        if ((!lr_given && !plain(args[8])) || !PyTuple_CheckExact(args[9]) || PyTuple_GET_SIZE(args[9]) != 2 || !number(PyTuple_GET_ITEM(args[9], 0), &options.beta1)
             || !number(PyTuple_GET_ITEM(args[9], 1), &options.beta2) || !number(args[10], &options.eps) || !number(args[7], &bits) || !number(args[11], &seed))
             Py_RETURN_NONE;
         options.bits = static_cast<int32_t>(bits);
@@ -284,6 +285,11 @@ PyObject* adamw_update(PyObject*, PyObject* const* args, Py_ssize_t count) {
             const at::Tensor& scale = THPVariable_Unpack(args[12]);
             if (scale.scalar_type() != at::kFloat || scale.numel() != 1 || scale.device() != device) Py_RETURN_NONE;
             options.scale_at = scale.data_ptr<float>();
+        }
+        if (!lr_given) {
+            const at::Tensor& lr = THPVariable_Unpack(args[8]);
+            if (lr.scalar_type() != at::kFloat || lr.numel() != 1 || lr.device() != device) Py_RETURN_NONE;
+            options.lr_at = lr.data_ptr<float>();
         }
         for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[6]); ++i) {
             if (!plain(PyTuple_GET_ITEM(args[6], i))) Py_RETURN_NONE;

@@ -29,6 +29,13 @@ from .frontend import capture
 from .passes import split_at_gradients
 
 
+def _refuse_operators(program: Any) -> None:
+    """A sharded step launches its own kernels; the calls of `losses.py` between them are not part of it."""
+    from .segments import has_operators
+    if has_operators(program):
+        raise ValueError("trainkernel: a sharded step cannot call the token operators (losses.py); use compile_training on one GPU")
+
+
 class PeerFailure(RuntimeError):
     """A peer rank reported a failure, or gave no sign of life within the limit."""
 
@@ -114,6 +121,7 @@ class ShardedTrainingStep:
             raise ValueError("trainkernel: the sharded step derives its own state mapping")
         self.group = group
         program, output_tree = capture(fn, example_inputs)
+        _refuse_operators(program)
         flat, self.input_tree = tree_flatten(tuple(example_inputs))
         state_leaves, _ = tree_flatten(example_inputs[0])
         n = self.count = len(state_leaves)
@@ -257,6 +265,7 @@ class FusedShardedTrainingStep:
         self.world = dist.get_world_size(group) if distributed else 1
         self.rank = dist.get_rank(group) if distributed else 0
         program, self.output_tree = capture(fn, example_inputs)
+        _refuse_operators(program)
         flat, self.input_tree = tree_flatten(tuple(example_inputs))
         state_leaves, _ = tree_flatten(example_inputs[0])
         n = self.count = len(state_leaves)

@@ -140,11 +140,14 @@ class AdamW:
             raise ValueError("trainkernel: AdamW: lr must be a non-negative number")
         if len(self.betas) != 2 or not all(number(b) and 0 <= b < 1 for b in self.betas):
             raise ValueError("trainkernel: AdamW: betas must be two numbers in [0, 1)")
-        if not number(self.eps) or not 0 < self.eps < float("inf"):
-            raise ValueError("trainkernel: AdamW: eps must be a positive number")
+        if not number(self.eps) or not 1e-30 <= self.eps < float("inf"):
+            raise ValueError("trainkernel: AdamW: eps must be a number of at least 1e-30")
         decays = (self.weight_decay,) if number(self.weight_decay) else self.weight_decay
         if isinstance(decays, str) or not all(number(w) and 0 <= w < float("inf") for w in decays):
             raise ValueError("trainkernel: AdamW: weight_decay must be a non-negative number, or one per tensor")
+        if not number(self.weight_decay):
+            object.__setattr__(self, "weight_decay", tuple(map(float, decays)))
+        object.__setattr__(self, "betas", tuple(self.betas))
         if self.state_bits not in (8, 32):
             raise ValueError("trainkernel: AdamW: state_bits must be 8 or 32")
         if isinstance(self.seed, bool) or not isinstance(self.seed, int) or not 0 <= self.seed < 2 ** 32:
@@ -165,6 +168,8 @@ class AdamW:
         self._decays(len(leaves))
         for leaf in leaves:
             self._check_param(leaf, device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("trainkernel: AdamW: init inside a stream capture would clear the moments in every replay")
         return AdamWState([leaf.numel() for leaf in leaves], self.state_bits, device)
 
     @staticmethod
@@ -225,4 +230,4 @@ class AdamW:
         for position, ((param_dtype, grad_dtype), items) in enumerate(groups.items()):
             operators.check(lib.tk_adamw_update((AdamWTensor * len(items))(*items), len(items), operators.DTYPES[param_dtype], operators.DTYPES[grad_dtype],
                                                 state._struct, options, int(position == len(groups) - 1), index, stream))
-        torch.autograd.graph.increment_version([*leaves, *state.tensors()])
+        torch.autograd.graph.increment_version([t for t in (*leaves, *state.tensors()) if not t.is_inference()])

@@ -180,6 +180,13 @@ class SegmentedProgram:
         for runner in self.kernels:
             runner.invalidate_carried()
 
+    def _single_only(self, *args: Any, **kwargs: Any) -> Any:
+        raise ValueError("trainkernel: a program that calls operators is several launches with buffers of their own; call it, or capture it")
+
+    allocate = run_into = _single_only
+    module = property(_single_only)
+    generated = property(_single_only)
+
     @staticmethod
     def _window(root: torch.Tensor, spec: TensorSpec) -> torch.Tensor:
         return root if tuple(root.shape) == spec.shape and tuple(root.stride()) == spec.strides and spec.offset == 0 else \
@@ -289,6 +296,16 @@ class OptimizedProgram:
 
     def status(self) -> Any:
         return self.runner.status()
+
+    def invalidate_carried(self) -> None:
+        self.runner.invalidate_carried()
+
+    allocate = run_into = SegmentedProgram._single_only
+    module = property(SegmentedProgram._single_only)
+
+    @property
+    def generated(self) -> Any:
+        return self.runner.generated
 
     def __call__(self, *inputs: torch.Tensor) -> tuple[torch.Tensor, ...]:
         self._validate_inputs(inputs)
