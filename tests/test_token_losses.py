@@ -246,11 +246,13 @@ def test_preference_loss_and_gradient(pairs, length, vocab, dtype, layout, maske
 
 
 @gpu
-def test_masked_vocabulary_and_extreme_logits():
+@pytest.mark.parametrize("vocab,times", [(1003, 1), (1003, 40), (40001, 1), (40001, 40), (70001, 40)])
+def test_masked_vocabulary_and_extreme_logits(vocab, times):
+    """Few rows and many, short and long: every block shape and the split rows."""
     lowest, inf = torch.finfo(BF16).min, float("inf")
     for dtype in (F32, BF16, F16):
         low = torch.finfo(dtype).min
-        rows = torch.zeros((6, 1003), dtype=dtype, device="cuda")
+        rows = torch.zeros((6, vocab), dtype=dtype, device="cuda")
         rows[0, 100:] = -inf                                   # part of the vocabulary excluded
         rows[1, :900] = low                                    # excluded with the type's lowest value, the target among them
         rows[2] = low                                          # everything excluded that way: uniform
@@ -259,12 +261,15 @@ def test_masked_vocabulary_and_extreme_logits():
         rows[5, 7] = inf
         targets = torch.tensor([3, 950, 10, 0, 1, 2], device="cuda")
         weights = torch.ones(6, device="cuda")
-        logp, grad = tk.token_logprobs_and_grad(rows, targets, weights)
+        every = tk.token_logprobs_and_grad(rows.repeat(times, 1), targets.repeat(times), weights.repeat(times))
+        logp, grad = every[0][-6:], every[1][-6:]
+        if times > 1:
+            assert torch.equal(every[0][:6].nan_to_num(), logp.nan_to_num()) and torch.equal(every[1][:6].nan_to_num(), grad.nan_to_num())
         want = torch.log_softmax(rows.double(), -1).gather(1, targets[:, None])[:, 0]
         assert bool(torch.isnan(want[4:]).all()) and bool(torch.isnan(logp[4:]).all())
-        torch.testing.assert_close(logp[:4].double(), want[:4], rtol=8 * U, atol=32 * U)
+        torch.testing.assert_close(logp[:4].double(), want[:4], rtol=8 * U, atol=(32 + vocab / 256) * U)
         expected = exact_grad(rows[:4], targets[:4], weights[:4].double())
-        torch.testing.assert_close(grad[:4].double(), expected, rtol=torch.finfo(dtype).eps / 2 + 32 * U, atol=torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps)
+        torch.testing.assert_close(grad[:4].double(), expected, rtol=torch.finfo(dtype).eps / 2 + (32 + vocab / 256) * U, atol=torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps)
         assert bool(torch.isnan(grad[4:]).all())
         # a target whose logit is -inf has log-probability -inf, and a gradient that is finite
         logp, grad = tk.token_logprobs_and_grad(rows[:1], torch.tensor([500], device="cuda"), weights[:1])

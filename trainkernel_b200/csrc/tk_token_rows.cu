@@ -278,6 +278,17 @@ __device__ __forceinline__ Parts parts_of(const T* x, int vocab) {
     return {head, (vocab - head) / kCount, (vocab - head) % kCount};
 }
 
+// A block's share of a row: all of it, or, where a cluster of blocks splits the row, an equal run of its vectors, with
+// the elements before and behind them in the first and the last block.
+struct Share {
+    int rank, size;
+    __device__ __forceinline__ int per(int vectors) const { return (vectors + size - 1) / size; }
+    __device__ __forceinline__ int begin(int vectors) const { return min(rank * per(vectors), vectors); }
+    __device__ __forceinline__ int end(int vectors) const { return min(rank * per(vectors) + per(vectors), vectors); }
+    __device__ __forceinline__ bool first() const { return rank == 0; }
+    __device__ __forceinline__ bool last() const { return rank == size - 1; }
+};
+
 // Loads that ask L2 to keep a line (it is read again soon) or to let go of it.
 __device__ __forceinline__ uint4 load_hint(const uint4* p, unsigned long long policy) {
     uint4 v;
@@ -295,11 +306,12 @@ constexpr int kAhead = 4;                      // vectors a thread has in flight
 // Statistics of a row.  The first `kept` vectors (a multiple of kAhead * THREADS, or the whole row) also go to shared
 // memory, where the thread that read them finds them again.
 template <typename T, int THREADS>
-__device__ __forceinline__ Stat row_stat(const T* x, int vocab, uint4* kept_at, int kept, bool again) {
+__device__ __forceinline__ Stat row_stat(const T* x, int vocab, const Share share, uint4* kept_at, int kept, bool again) {
     const Parts p = parts_of(x, vocab);
     const uint4* body = reinterpret_cast<const uint4*>(x + p.head);
     Stat s{kLowest, 0.f};
-    int i = threadIdx.x;
+    const int end = share.end(p.vectors);
+    int i = share.begin(p.vectors) + threadIdx.x;
     const int first = min(kept, p.vectors);
     for (; i + (kAhead - 1) * THREADS < first; i += kAhead * THREADS) {
         uint4 v[kAhead];
@@ -315,24 +327,24 @@ __device__ __forceinline__ Stat row_stat(const T* x, int vocab, uint4* kept_at, 
         accumulate<T, 1>(s, v);
     }
     const unsigned long long policy = keep_policy();
-    for (; i + (kAhead - 1) * THREADS < p.vectors; i += kAhead * THREADS) {
+    for (; i + (kAhead - 1) * THREADS < end; i += kAhead * THREADS) {
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) v[k] = again ? load_hint(body + i + k * THREADS, policy) : __ldcg(body + i + k * THREADS);
         accumulate<T, kAhead>(s, v);
     }
-    for (; i < p.vectors; i += THREADS) {
+    for (; i < end; i += THREADS) {
         const uint4 v[1] = {__ldcg(body + i)};
         accumulate<T, 1>(s, v);
     }
-    if (threadIdx.x < p.head) accumulate_one(s, x[threadIdx.x]);
-    if (threadIdx.x < p.tail) accumulate_one(s, x[vocab - p.tail + threadIdx.x]);
+    if (share.first() && threadIdx.x < p.head) accumulate_one(s, x[threadIdx.x]);
+    if (share.last() && threadIdx.x < p.tail) accumulate_one(s, x[vocab - p.tail + threadIdx.x]);
     return s;
 }
 
 // coefficient * (delta - p) for every logit of a row; `factor` = -coefficient / sum.
 template <typename T, int THREADS>
-__device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int target, const Exponent e, float factor, float coefficient, bool in_phase,
+__device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, const Share share, int target, const Exponent e, float factor, float coefficient, bool in_phase,
                                          const uint4* kept_at, int kept) {
     const auto one = [&](int j) {
         float value = exp2_fast(e(Vector<T>::load(x[j]))) * factor;
@@ -340,7 +352,7 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int targ
         out[j] = Vector<T>::store(value);
     };
     if (!in_phase || e.extreme) {
-        for (int j = threadIdx.x; j < vocab; j += THREADS) one(j);
+        for (int64_t j = threadIdx.x + share.rank * THREADS; j < vocab; j += THREADS * share.size) one(static_cast<int>(j));
         return;
     }
     constexpr int kCount = Vector<T>::kCount, kPairs = kCount / 2;
@@ -367,8 +379,8 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int targ
         __stcs(to + i, Vector<T>::pack(f));
     };
     // From the row's end, which was read last and is near, to the part kept in shared memory.
-    const int first = min(kept, p.vectors), left = (p.vectors - first) % (kAhead * THREADS);
-    for (int i = p.vectors - kAhead * THREADS + threadIdx.x; i >= first + left; i -= kAhead * THREADS) {
+    const int end = share.end(p.vectors), first = kept ? min(kept, p.vectors) : share.begin(p.vectors), left = (end - first) % (kAhead * THREADS);
+    for (int i = end - kAhead * THREADS + threadIdx.x; i >= first + left; i -= kAhead * THREADS) {
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) v[k] = __ldcs(body + i + k * THREADS);
@@ -376,18 +388,19 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, int targ
         for (int k = 0; k < kAhead; ++k) vector(i + k * THREADS, v[k]);
     }
     for (int i = first + threadIdx.x; i < first + left; i += THREADS) vector(i, __ldcs(body + i));
-    for (int i = threadIdx.x; i < first; i += THREADS) vector(i, kept_at[i]);
-    if (threadIdx.x < p.head) one(threadIdx.x);
-    if (threadIdx.x < p.tail) one(vocab - p.tail + threadIdx.x);
+    if (kept)
+        for (int i = threadIdx.x; i < first; i += THREADS) vector(i, kept_at[i]);
+    if (share.first() && threadIdx.x < p.head) one(threadIdx.x);
+    if (share.last() && threadIdx.x < p.tail) one(vocab - p.tail + threadIdx.x);
 }
 
 template <typename T, int THREADS>
-__device__ __forceinline__ void row_zero(T* out, int vocab) {
+__device__ __forceinline__ void row_zero(T* out, int vocab, const Share share) {
     const Parts p = parts_of(out, vocab);
     uint4* to = reinterpret_cast<uint4*>(out + p.head);
-    for (int i = threadIdx.x; i < p.vectors; i += THREADS) __stcs(to + i, make_uint4(0, 0, 0, 0));
-    if (threadIdx.x < p.head) out[threadIdx.x] = Vector<T>::store(0.f);
-    if (threadIdx.x < p.tail) out[vocab - p.tail + threadIdx.x] = Vector<T>::store(0.f);
+    for (int i = share.begin(p.vectors) + threadIdx.x; i < share.end(p.vectors); i += THREADS) __stcs(to + i, make_uint4(0, 0, 0, 0));
+    if (share.first() && threadIdx.x < p.head) out[threadIdx.x] = Vector<T>::store(0.f);
+    if (share.last() && threadIdx.x < p.tail) out[vocab - p.tail + threadIdx.x] = Vector<T>::store(0.f);
 }
 
 // Kernels that follow another one of the same call are launched while it still runs and wait here for its results.
@@ -416,21 +429,43 @@ __device__ __forceinline__ void sum_terms(const float* terms, int64_t rows, floa
     }
 }
 
-template <typename T, Mode MODE, Loss LOSS, int THREADS, int BLOCKS>
+constexpr int kMostShares = 8;                 // blocks of a cluster
+
+// The statistics of all blocks of a cluster, in every thread: each block writes its own into every block's shared memory.
+__device__ __forceinline__ Stat cluster_join(Stat mine, const Share share, float2* parts) {
+    if (threadIdx.x < share.size) {
+        uint32_t to;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(parts + share.rank))), "r"(threadIdx.x));
+        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to), "l"(pair(mine.top, mine.sum)) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int lane = threadIdx.x % 32;
+    const float2 part = lane < share.size ? parts[lane] : make_float2(kLowest, 0.f);
+    return warp_join({part.x, part.y});
+}
+
+// One block per row, or, with SPLIT, one cluster of blocks per row.
+template <typename T, Mode MODE, Loss LOSS, int THREADS, int BLOCKS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __grid_constant__ Args a, const int kept) {
     extern __shared__ uint4 kept_at[];
     __shared__ Stat shared[32];
     __shared__ float shared_coefficient;
     __shared__ bool shared_last;
+    __shared__ float2 shared_parts[SPLIT ? kMostShares : 1];
     const tk_token_rows& r = a.rows;
-    const int64_t row = blockIdx.x, b = row / r.length, t = row % r.length;
+    Share share{0, 1};
+    if (SPLIT) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(share.rank));
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(share.size));
+    }
+    const int64_t row = blockIdx.x / static_cast<unsigned>(share.size), b = row / r.length, t = row % r.length;
     const T* x = static_cast<const T*>(r.logits) + b * r.stride_batch + t * r.stride_token;
     T* out = static_cast<T*>(a.grad.data) + b * a.grad.stride_batch + t * a.grad.stride_token;
     const bool keep = counts(r, b, t);
     const int vocab = static_cast<int>(r.vocab);
     Stat stat{kLowest, 0.f};
     int target = -1;
-    if (a.clear && row == 0 && threadIdx.x == 0) *a.clear = 0;
+    if (a.clear && blockIdx.x == 0 && threadIdx.x == 0) *a.clear = 0;
     if (keep) {
         const int64_t wanted = target_of(r, b, t);
         target = wanted >= 0 && wanted < vocab ? static_cast<int>(wanted) : -1;
@@ -452,11 +487,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __gri
     }
     if (MODE == kGrad) wait_for_previous();
     if (MODE != kStats && LOSS != kPolicy && keep) weight = at(a.coefficients, b, t);
-    if (MODE != kGrad && keep) stat = block_join<THREADS>(row_stat<T, THREADS>(x, vocab, kept_at, kept, MODE == kBoth), shared);
+    if (MODE != kGrad && keep) {
+        stat = block_join<THREADS>(row_stat<T, THREADS>(x, vocab, share, kept_at, kept, MODE == kBoth), shared);
+        if (SPLIT) stat = cluster_join(stat, share, shared_parts);
+    }
     if (MODE != kGrad && threadIdx.x == 0) {
         const float logprob = keep ? row_logprob(stat, value) : 0.f;
-        if (a.logprobs) a.logprobs[row] = logprob;
-        if (a.stats) {
+        if (share.first() && a.logprobs) a.logprobs[row] = logprob;
+        if (share.first() && a.stats) {
             a.stats[2 * row] = stat.top;
             a.stats[2 * row + 1] = stat.sum;
         }
@@ -469,8 +507,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __gri
                 term *= weight;
                 slope *= weight;
             }
-            a.terms[row] = term;
-            if (a.row_coefficients) a.row_coefficients[row] = slope;
+            if (share.first()) {
+                a.terms[row] = term;
+                if (a.row_coefficients) a.row_coefficients[row] = slope;
+            }
             shared_coefficient = slope;
         }
     }
@@ -485,16 +525,16 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __gri
             }
             if (MODE == kGrad) stat = {a.stats[2 * row], a.stats[2 * row + 1]};
             const float factor = target >= 0 ? -coefficient / stat.sum : not_a_number();
-            row_grad<T, THREADS>(out, x, vocab, target, Exponent(stat.top), factor, coefficient, a.in_phase, kept_at, kept);
+            row_grad<T, THREADS>(out, x, vocab, share, target, Exponent(stat.top), factor, coefficient, a.in_phase, kept_at, kept);
         } else {
-            row_zero<T, THREADS>(out, vocab);
+            row_zero<T, THREADS>(out, vocab, share);
         }
     }
-    if (MODE != kGrad && LOSS == kPolicy && a.counter) {
+    if (MODE != kGrad && LOSS == kPolicy && a.counter && share.first()) {
         // The block that finishes last adds the terms of all rows.
         if (threadIdx.x == 0) {
             __threadfence();
-            shared_last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
+            shared_last = atomicAdd(a.counter, 1u) == gridDim.x / share.size - 1;
             __threadfence();
         }
         __syncthreads();
@@ -591,19 +631,33 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int64_t pairs, in
 
 // `early`: the kernel may start while the previous one of this call runs; it waits for it itself.
 template <typename... A>
-int launch(void (*kernel)(A...), int64_t grid, int threads, size_t shared, bool early, cudaStream_t stream, A... arguments) {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+int launch_clusters(void (*kernel)(A...), int64_t grid, int cluster, int threads, size_t shared, bool early, cudaStream_t stream, A... arguments) {
+    cudaLaunchAttribute attributes[2] = {};
+    int count = 0;
+    if (early) {
+        attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[count++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attributes[count].id = cudaLaunchAttributeClusterDimension;
+        attributes[count].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attributes[count].val.clusterDim.y = attributes[count].val.clusterDim.z = 1;
+        ++count;
+    }
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(grid));
     config.blockDim = dim3(static_cast<unsigned>(threads));
     config.dynamicSmemBytes = shared;
     config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = early ? 1 : 0;
+    config.attrs = attributes;
+    config.numAttrs = static_cast<unsigned>(count);
     count_launch();
     return check(cudaLaunchKernelEx(&config, kernel, arguments...), "launching a token kernel");
+}
+
+template <typename... A>
+int launch(void (*kernel)(A...), int64_t grid, int threads, size_t shared, bool early, cudaStream_t stream, A... arguments) {
+    return launch_clusters(kernel, grid, 1, threads, shared, early, stream, arguments...);
 }
 
 constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
@@ -616,10 +670,15 @@ constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
 template <typename T, Mode MODE, Loss LOSS>
 int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
     const int64_t bytes = a.rows.vocab * static_cast<int64_t>(sizeof(T)), grid = a.rows.batch * a.rows.length;
-    if (bytes <= 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 128, 16>, grid, 128, 0, early, stream, a, 0);
-    if (MODE != kBoth) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3>, grid, 512, 0, early, stream, a, 0);
-    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 5>, grid, 256, 0, early, stream, a, 0);
-    auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2>;
+    // Fewer rows than multiprocessors: clusters of blocks split them, as long as a block has 8 KB to read.
+    const int sms = tk_ops::sm_count(device);
+    int shares = 1;
+    while (shares < kMostShares && grid * shares * 2 <= sms && bytes / (shares * 2) >= 8 * 1024) shares *= 2;
+    if (shares > 1) return launch_clusters(token_rows_kernel<T, MODE, LOSS, 256, 2, true>, grid * shares, shares, 256, 0, early, stream, a, 0);
+    if (bytes <= 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 128, 16, false>, grid, 128, 0, early, stream, a, 0);
+    if (MODE != kBoth) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
+    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 5, false>, grid, 256, 0, early, stream, a, 0);
+    auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2, false>;
     static std::atomic<bool> sized[64];
     if (device >= 64 || !sized[device].load(std::memory_order_relaxed)) {
         if (int code = check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptVectors * 16), "sizing shared memory")) return code;
