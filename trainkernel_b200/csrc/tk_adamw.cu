@@ -162,11 +162,13 @@ template <typename T> __device__ __forceinline__ void store8(T* to, const float 
 }
 
 __device__ __forceinline__ void decode8(float (&to)[8], uint2 codes, float scale) {
+    const Pair scales = pair(scale, scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t byte = ((i < 4 ? codes.x : codes.y) >> (8 * (i % 4))) & 0xff;
-        const __half_raw half = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
-        to[i] = __fmul_rn(__half2float(__half(half)), scale);
+    for (int i = 0; i < 8; i += 2) {
+        const uint32_t two = (i < 4 ? codes.x : codes.y) >> (8 * (i % 4));
+        const __half2_raw halves = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+        const float2 values = __half22float2(__half2(halves));
+        split(mul2(pair(values.x, values.y), scales), to[i], to[i + 1]);
     }
 }
 
@@ -243,9 +245,9 @@ __device__ __forceinline__ void update8(const tk_adamw_state& state, const Item&
         a = sqrtf(v[i]);
         b = sqrtf(v[i + 1]);
         split(fma2(pair(a, b), n.spread, n.eps), c, d);
-        // p decay - pace m / (sqrt(v) spread + eps)
+        // p decay - pace m / (sqrt(v) spread + eps); n.pace is negative
         const Pair change = mul2(mul2(n.pace, mean), pair(reciprocal(c), reciprocal(d)));
-        split(fma2(pair(p[i], p[i + 1]), decays, change ^ 0x8000000080000000ull), p[i], p[i + 1]);
+        split(fma2(pair(p[i], p[i + 1]), decays, change), p[i], p[i + 1]);
         if (BITS == 8) {
             v[i] = a;
             v[i + 1] = b;
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
     n.scale = pair(scale, scale);
     n.spread = pair(spread, spread);
     n.eps = pair(a.eps, a.eps);
-    n.pace = pair(pace, pace);
+    n.pace = pair(-pace, -pace);
     n.salt = mix(static_cast<uint32_t>(step) + a.seed * 0x9e3779b9u);
 
     // Chunks are dealt out one by one, so that blocks that run together touch neighbouring memory (contiguous runs per
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
 }
 
 template <typename P, typename G, int BITS, int CAPACITY>
-int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, cudaStream_t stream) {
+int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int device, cudaStream_t stream) {
     Args<CAPACITY> a;
     a.state = *state;
     a.lr_at = o->lr_at;
@@ -371,9 +373,17 @@ int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* stat
         if (chunks > 0x7fffffff) return fail(TK_E_ARGUMENT, "trainkernel: too many elements in one tk_adamw_update");
     }
     a.chunks = static_cast<int32_t>(chunks);
-    // Several waves, so that the hardware evens out what blocks take (33.5M elements, 32-bit moments: 170 us with one wave
-    // of 592 blocks, 164 with two, 157 with three, 148 with six).
+    // 32-bit moments are bound by memory: as many blocks as there are counters, so that the hardware evens out what they take
+    // (33.5M elements: 170 us with one wave of 592 blocks, 164 with two, 157 with three, 148 with six).  8-bit moments
+    // are bound by arithmetic, a block's start-up counts, and whole waves of four chunks or more a block are best (8.4M
+    // elements: 24.7 us with one wave, 28.3 with a block per chunk, 30.4 with 1.2 waves; 33.5M: 101 with 2.3, 93 with seven).
     int64_t grid = chunks;
+    const int64_t wave = 4 * static_cast<int64_t>(tk_ops::sm_count(device));
+    if (BITS == 8 && wave > 0) {
+        const int64_t waves = chunks / (4 * wave);
+        grid = wave * (waves < 1 ? 1 : waves > 6 ? 6 : waves);
+        if (grid > chunks) grid = chunks;
+    }
     if (grid > TK_ADAMW_COUNTERS) grid = TK_ADAMW_COUNTERS;
     if (grid > chunks) grid = chunks;
     if (grid < 1) grid = 1;
@@ -383,27 +393,27 @@ int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* stat
 }
 
 template <typename P, typename G, int BITS>
-int launch_all(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, cudaStream_t stream) {
+int launch_all(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* state, const tk_adamw_options* o, int last, int device, cudaStream_t stream) {
     while (count > kMany) {
-        if (int code = launch<P, G, BITS, kMany>(tensors, kMany, state, o, 0, stream)) return code;
+        if (int code = launch<P, G, BITS, kMany>(tensors, kMany, state, o, 0, device, stream)) return code;
         tensors += kMany;
         count -= kMany;
     }
-    return count > kFew ? launch<P, G, BITS, kMany>(tensors, count, state, o, last, stream)
-                        : launch<P, G, BITS, kFew>(tensors, count, state, o, last, stream);
+    return count > kFew ? launch<P, G, BITS, kMany>(tensors, count, state, o, last, device, stream)
+                        : launch<P, G, BITS, kFew>(tensors, count, state, o, last, device, stream);
 }
 
 template <typename P, typename G>
-int by_bits(const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, cudaStream_t stream) {
-    return o->bits == 8 ? launch_all<P, G, 8>(t, n, s, o, last, stream) : launch_all<P, G, 32>(t, n, s, o, last, stream);
+int by_bits(const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int device, cudaStream_t stream) {
+    return o->bits == 8 ? launch_all<P, G, 8>(t, n, s, o, last, device, stream) : launch_all<P, G, 32>(t, n, s, o, last, device, stream);
 }
 
 template <typename P>
-int by_grad(int dtype, const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, cudaStream_t stream) {
+int by_grad(int dtype, const tk_adamw_tensor* t, int n, const tk_adamw_state* s, const tk_adamw_options* o, int last, int device, cudaStream_t stream) {
     switch (dtype) {
-        case TK_F32: return by_bits<P, float>(t, n, s, o, last, stream);
-        case TK_F16: return by_bits<P, __half>(t, n, s, o, last, stream);
-        default: return by_bits<P, __nv_bfloat16>(t, n, s, o, last, stream);
+        case TK_F32: return by_bits<P, float>(t, n, s, o, last, device, stream);
+        case TK_F16: return by_bits<P, __half>(t, n, s, o, last, device, stream);
+        default: return by_bits<P, __nv_bfloat16>(t, n, s, o, last, device, stream);
     }
 }
 
@@ -424,8 +434,8 @@ extern "C" int tk_adamw_update(const tk_adamw_tensor* tensors, int count, int pa
     if (scope.status) return scope.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (param_dtype) {
-        case TK_F32: return by_grad<float>(grad_dtype, tensors, count, state, options, last, s);
-        case TK_F16: return by_grad<__half>(grad_dtype, tensors, count, state, options, last, s);
-        default: return by_grad<__nv_bfloat16>(grad_dtype, tensors, count, state, options, last, s);
+        case TK_F32: return by_grad<float>(grad_dtype, tensors, count, state, options, last, device, s);
+        case TK_F16: return by_grad<__half>(grad_dtype, tensors, count, state, options, last, device, s);
+        default: return by_grad<__nv_bfloat16>(grad_dtype, tensors, count, state, options, last, device, s);
     }
 }
