@@ -328,6 +328,26 @@ def test_parameters_on_the_host_are_refused():
 
 
 @gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_continues_where_it_was_taken(bits, tmp_path):
+    sizes = [700, 3]
+    p, g = tensors(sizes, F32, 1.0, 70), tensors(sizes, F32, 0.1, 71)
+    optimizer = tk.AdamW(state_bits=bits)
+    state = optimizer.init(p)
+    optimizer.update(p, g, state)
+    torch.save((p, state.state_dict()), tmp_path / "checkpoint")
+    optimizer.update(p, g, state)
+    q, saved = torch.load(tmp_path / "checkpoint", weights_only=False)
+    other = optimizer.init(q)
+    other.load_state_dict(saved)
+    optimizer.update(q, g, other)
+    for a, b in zip([*p, *state.tensors()], [*q, *other.tensors()]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    with pytest.raises(ValueError, match="other tensors"):
+        optimizer.init(q[:1]).load_state_dict(saved)
+
+
+@gpu
 def test_init_inside_a_capture_is_refused():
     p = [torch.zeros(4, device="cuda")]
     tk.AdamW().init(p)

@@ -76,6 +76,17 @@ class AdamWState:
             return (self.exp_avg, self.exp_avg_sq, self._counters)
         return (self.exp_avg, self.exp_avg_root, self.exp_avg_scale, self.exp_avg_root_scale, self._counters)
 
+    def state_dict(self) -> dict[str, Any]:
+        """Copies of the moments with the sizes they belong to, for a checkpoint."""
+        return {"sizes": self.sizes, "bits": self.bits, "tensors": tuple(t.clone() for t in self.tensors())}
+
+    def load_state_dict(self, saved: dict[str, Any]) -> None:
+        """Take over what `state_dict` of a state of the same sizes and bits returned."""
+        if tuple(saved["sizes"]) != self.sizes or saved["bits"] != self.bits:
+            raise ValueError("trainkernel: AdamW: the saved state belongs to other tensors or another number of bits")
+        for mine, theirs in zip(self.tensors(), saved["tensors"]):
+            mine.copy_(theirs)
+
     def moments(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
         """First and second moment of tensor `index` as flat FP32 tensors."""
         begin, size = self.offsets[index], self.sizes[index]
