@@ -62,6 +62,7 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
 template <typename T> struct Vector;
 template <> struct Vector<float> {
     static constexpr int kCount = 4;
+    static constexpr bool kSplit = false;          // whether gradients need exp2_split
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[2]) {
         f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
         f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
@@ -77,6 +78,7 @@ template <> struct Vector<float> {
 };
 template <> struct Vector<__nv_bfloat16> {
     static constexpr int kCount = 8;
+    static constexpr bool kSplit = false;
     static __device__ __forceinline__ float2 two(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
         f[0] = two(v.x);
@@ -99,6 +101,7 @@ template <> struct Vector<__nv_bfloat16> {
 };
 template <> struct Vector<__half> {
     static constexpr int kCount = 8;
+    static constexpr bool kSplit = true;
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
         const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
@@ -146,6 +149,15 @@ __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float x = e.extreme ? (a.top - top) * kLog2e : scaled(a.top) - e.base;
     const float y = e.extreme ? (b.top - top) * kLog2e : scaled(b.top) - e.base;
     return {top, a.sum * exp2_fast(x) + b.sum * exp2_fast(y)};
+}
+
+// 2^(x log2(e) - base) with the exponent split at a whole number, so that its fraction keeps all of its bits: the rounding of
+// an exponent near -12 alone costs 2^-21 of the value, more than one part in a hundred of half a step of FP16, and with small
+// gradients, which FP16 holds in few bits, would tip several times as many of them to the other side as FP32's exp does.
+__device__ __forceinline__ float exp2_split(float x, float base) {
+    const float whole = fmaxf(fmaf(x, kLog2e, -base), -126.f) + 12582912.f;           // 1.5 2^23: rounded to a whole number
+    const float n = whole - 12582912.f;
+    return exp2_fast(fmaf(x, kLog2e, -(base + n))) * __int_as_float((__float_as_int(whole) << 23) + 0x3f800000);
 }
 
 // Adds N vectors of logits to a thread's statistics.
@@ -302,6 +314,18 @@ __device__ __forceinline__ unsigned long long keep_policy() {
 
 constexpr int kAhead = 4;                      // vectors a thread has in flight
 
+// Asks L2 for the vectors of a thread's next turn before it loads those of this one: registers for a second set in flight
+// would cost resident blocks.  8000 x 32000 BF16 logits with gradient: 198 -> 179 us; two or three turns ahead 186 and 190.
+template <int THREADS>
+__device__ __forceinline__ void prefetch_turn(const uint4* body, int i, int end) {
+    if (threadIdx.x % 8) return;                           // one request for every 128 bytes
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const int next = i + (kAhead + k) * THREADS;
+        if (next < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(body + next));
+    }
+}
+
 // Statistics of a row, or of a block's share of it.  The first `kept` vectors of a whole row also go to shared memory, where
 // the thread that read them finds them again; of the rest L2 is asked to keep what is read `again`.
 template <typename T, int THREADS>
@@ -313,6 +337,7 @@ __device__ __forceinline__ Stat row_stat(const T* x, int vocab, const Share shar
     int i = share.begin(p.vectors) + threadIdx.x;
     const int first = min(kept, p.vectors);
     for (; i + (kAhead - 1) * THREADS < first; i += kAhead * THREADS) {
+        prefetch_turn<THREADS>(body, i, end);
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) v[k] = __ldcs(body + i + k * THREADS);
@@ -327,6 +352,7 @@ __device__ __forceinline__ Stat row_stat(const T* x, int vocab, const Share shar
     }
     const unsigned long long policy = keep_policy();
     for (; i + (kAhead - 1) * THREADS < end; i += kAhead * THREADS) {
+        prefetch_turn<THREADS>(body, i, end);
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) v[k] = again ? load_hint(body + i + k * THREADS, policy) : __ldcg(body + i + k * THREADS);
@@ -346,7 +372,8 @@ template <typename T, int THREADS>
 __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, const Share share, int target, const Exponent e, float factor, float coefficient, bool in_phase,
                                          const uint4* kept_at, int kept) {
     const auto one = [&](int j) {
-        float value = exp2_fast(e(Vector<T>::load(x[j]))) * factor;
+        const float logit = Vector<T>::load(x[j]);
+        float value = (Vector<T>::kSplit && !e.extreme ? exp2_split(logit, e.base) : exp2_fast(e(logit))) * factor;
         if (j == target) value += coefficient;
         out[j] = Vector<T>::store(value);
     };
@@ -365,8 +392,12 @@ __device__ __forceinline__ void row_grad(T* out, const T* x, int vocab, const Sh
         Vector<T>::unpack(v, f);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
-            const float2 y = both(fma2(pair(f[k].x, f[k].y), scale, base));
-            f[k] = both(mul2(pair(exp2_fast(y.x), exp2_fast(y.y)), by));
+            if (Vector<T>::kSplit) {
+                f[k] = both(mul2(pair(exp2_split(f[k].x, e.base), exp2_split(f[k].y, e.base)), by));
+            } else {
+                const float2 y = both(fma2(pair(f[k].x, f[k].y), scale, base));
+                f[k] = both(mul2(pair(exp2_fast(y.x), exp2_fast(y.y)), by));
+            }
         }
         if (i == special) {
 #pragma unroll
@@ -447,10 +478,9 @@ __device__ __forceinline__ Stat cluster_join(Stat mine, const Share share, float
     return warp_join({part.x, part.y});
 }
 
-// One block per row, or, with SPLIT, one cluster of blocks per row.  The statistics alone (8192 rows of 128256 BF16 logits)
-// take 352 us, 97 % of the copy rate in a loop of 4096 rows: memory bounds them, with the exponential unit 72 % busy.  With
-// the gradient the same rows take 683 us where reading and writing them takes 562: between the passes a block waits for
-// its join, and only the other blocks of the multiprocessor fill that time (see launch_type for the block shapes).
+// One block per row, or, with SPLIT, one cluster of blocks per row.  Memory bounds the statistics alone; with the gradient a
+// block waits for its join between the passes, which only the other blocks of the multiprocessor fill, and every logit
+// takes two exponentials (65 % of their unit at 8000 x 32000 BF16).  launch_type has the block shapes and their times.
 template <typename T, Mode MODE, Loss LOSS, int THREADS, int BLOCKS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __grid_constant__ Args a, const int kept) {
     extern __shared__ uint4 kept_at[];
@@ -669,11 +699,14 @@ int launch(void (*kernel)(A...), int64_t grid, int threads, size_t shared, bool 
 
 constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
 
-// How many threads share a row, and so how many rows are in flight.  More, smaller blocks hide one another's joins:
-// 16384 x 8000 BF16 logits with gradient take 126 us with 16 blocks of 128 threads on an SM, 134 with 12, 149 with 8; rows
-// of 62 KB take 205 us (8000 of them) with 5 blocks of 256 threads, 234 with 4 and 314 with 2 of 640.  For long rows the
-// second read has to find the row in L2, and few rows may be in flight: 4096 rows of 250 KB take 388 us with 2 blocks of
-// 640 threads that keep the first 80 KB of their row in shared memory, 417 without keeping it, 444 with 3 of 512.
+// How many threads share a row, and so how many rows are in flight.  More, smaller blocks hide one another's joins until
+// registers run out: 16384 x 8000 BF16 logits with gradient take 106 us with 18 blocks of 96 threads on an SM, 111 with 24 of
+// 64, 116 with 16 of 128, 149 with 8 of 256; rows of 62 KB (8000 of them) take 176 us with 6 blocks of 256 threads, 179 with
+// 5, 185 with 4, 194 with 8 of 192, 196 with 3 of 512.  For long rows the second read has to find the row in L2, so few rows
+// may be in flight: 4096 rows of 250 KB take 363 us with 2 blocks of 640 threads that keep the first 80 KB of their row in
+// shared memory; before L2 was asked ahead 394, 417 without keeping, 444 with 3 blocks of 512.  The statistics alone take
+// 158 us of those rows with 3 blocks of 512 threads, 161 with 6 of 256, 176 with 8 of 256.  Short rows that all run at once
+// get more threads each (256 x 1000 FP32 with gradient, captured: 7.0 us with 256, 7.2 with 128, 8.7 with 96).
 template <typename T, Mode MODE, Loss LOSS>
 int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
     const int64_t bytes = a.rows.vocab * static_cast<int64_t>(sizeof(T)), grid = a.rows.batch * a.rows.length;
@@ -682,9 +715,9 @@ int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
     int shares = 1;
     while (shares < kMostShares && grid * shares * 2 <= sms && bytes / (shares * 2) >= 8 * 1024) shares *= 2;
     if (shares > 1) return launch_clusters(token_rows_kernel<T, MODE, LOSS, 256, 2, true>, grid * shares, shares, 256, 0, early, stream, a, 0);
-    if (bytes <= 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 128, 16, false>, grid, 128, 0, early, stream, a, 0);
-    if (MODE != kBoth) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
-    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 5, false>, grid, 256, 0, early, stream, a, 0);
+    if (bytes <= 16 * 1024 && grid > 4 * sms) return launch(token_rows_kernel<T, MODE, LOSS, 96, 18, false>, grid, 96, 0, early, stream, a, 0);
+    if (MODE != kBoth && bytes > 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
+    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 6, false>, grid, 256, 0, early, stream, a, 0);
     auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2, false>;
     static std::atomic<bool> sized[64];
     if (device >= 64 || !sized[device].load(std::memory_order_relaxed)) {
