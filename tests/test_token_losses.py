@@ -350,7 +350,7 @@ def test_the_three_ways_to_a_gradient_agree():
     # the same coefficients and statistics, added in the same order: at most the rounding of one product apart
     for other in (transformed, leaf.grad):
         torch.testing.assert_close(other.float(), grad.float(), rtol=torch.finfo(BF16).eps, atol=1e-30)
-    assert abs(float(value) / 3 - float(loss)) <= 4 * U * abs(float(loss))
+    assert abs(float(value.detach()) / 3 - float(loss)) <= 4 * U * abs(float(loss))
     leaf.grad = None
     out = tk.token_logprobs(leaf, targets, mask=mask)
     weights = noise((3, 5), 1.0, 21)
@@ -505,6 +505,47 @@ def test_transformed_constants_are_refused():
     logits, targets, _ = make((3,), 20, F32, 44)
     with pytest.raises(ValueError, match="detach"):
         torch.func.grad(lambda a: tk.policy_loss_and_grad(logits, targets, torch.zeros(3, device="cuda"), a)[0])(torch.ones(3, device="cuda"))
+
+
+@gpu
+def test_gradients_behind_two_to_the_31_elements():
+    rows, vocab = 20000, 120000                               # 2.4e9 logits, 4.8 GB, and as much for the gradient
+    logits = torch.empty((rows, vocab), dtype=BF16, device="cuda")
+    logits.normal_(0.0, 2.0, generator=torch.Generator(device="cuda").manual_seed(45))
+    targets = torch.randint(0, vocab, (rows,), device="cuda")
+    mask = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    mask[::997] = mask[-3:] = True
+    logp, grad = tk.token_logprobs_and_grad(logits, targets, torch.ones(1, device="cuda"), mask=mask)
+    at = torch.nonzero(mask)[:, 0]
+    assert_logprobs(logp[at], logits[at], targets[at])
+    assert_grad(grad[at], logits[at], targets[at], torch.ones(len(at), dtype=torch.float64, device="cuda"), 2 * U)
+    assert bool((grad[-5] == 0).all()) and bool((logp[~mask] == 0).all())
+
+
+@gpu
+def test_inference_mode_and_parameters_as_logits():
+    logits, targets, _ = make((6,), 700, F32, 46)
+    want = tk.token_logprobs(logits, targets)
+    with torch.inference_mode():
+        assert torch.equal(tk.token_logprobs(logits, targets), want)
+        inside = logits.clone()
+        assert torch.equal(tk.token_logprobs(inside, targets), want)
+        assert torch.equal(tk.policy_loss_and_grad(inside, targets, want, want)[1], want)
+    leaf = torch.nn.Parameter(logits)
+    with torch.no_grad():
+        assert not tk.token_logprobs(leaf, targets).requires_grad
+    assert not tk.token_logprobs_and_grad(leaf, targets, want)[1].requires_grad
+    assert tk.token_logprobs(leaf, targets).requires_grad
+
+
+@gpu
+def test_logits_of_one_element_of_memory():
+    """Expanded logits: every row the same memory; the gradient has memory of its own."""
+    base = torch.randn((1, 1, 300), device="cuda")
+    logits, targets = base.expand(3, 4, 300), torch.randint(0, 300, (3, 4), device="cuda")
+    logp, grad = tk.token_logprobs_and_grad(logits, targets, torch.ones(4, device="cuda"))
+    assert_logprobs(logp, logits, targets)
+    assert_grad(grad, logits, targets, torch.ones((3, 4), dtype=torch.float64, device="cuda"), 2 * U)
 
 
 # -- refusals (no GPU) ---------------------------------------------------------------------------------------

@@ -20,7 +20,6 @@ No counterpart in the reference, whose losses are means of squares (reference: b
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
