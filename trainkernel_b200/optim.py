@@ -197,7 +197,7 @@ class AdamW:
     def update(self, params: Any, grads: Any, state: AdamWState, *, grad_scale: torch.Tensor | None = None) -> None:
         """One step, in place, on the current stream.
 
-        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16).  `grad_scale` (one FP32 value on the
+        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16); parameters do not overlap.  `grad_scale` (one FP32 value on the
         device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
         not happen: parameters, moments and step count stay as they are.
         """
