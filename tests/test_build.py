@@ -35,3 +35,33 @@ def test_kernels_are_built_without_a_tests_package(monkeypatch, tmp_path):
         monkeypatch.delitem(sys.modules, name)
     monkeypatch.setitem(sys.modules, "tests", None)
     assert prebuilt(monkeypatch, tmp_path) > 10
+
+
+# -- without the operators' compiled host path -------------------------------------------------------------------
+
+def no_host_path(*_, **__):
+    raise RuntimeError("trainkernel: building the operators' host path failed:\nno headers")
+
+
+def test_build_goes_on_without_the_host_path(monkeypatch, capsys):
+    from trainkernel_b200 import noalloc, operators
+    for module, name in ((runtime, "build_library"), (runtime, "library"), (noalloc, "build_library"), (operators, "build_library")):
+        monkeypatch.setattr(module, name, lambda **_: None)
+    monkeypatch.setattr(operators, "build_host", no_host_path)
+    monkeypatch.setattr(entry, "_prebuild_kernels", lambda: 7)
+    entry.build()
+    said = capsys.readouterr().out
+    assert "host path skipped" in said and "7 sm_100a kernels" in said
+
+
+def test_operators_run_without_the_host_path(monkeypatch):
+    import torch
+    from trainkernel_b200 import operators
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda index: (10, 0))
+    monkeypatch.setattr(operators, "_usable", {})
+    monkeypatch.setattr(operators, "fast", None)
+    monkeypatch.setattr(operators, "_host", None)
+    monkeypatch.setattr(operators, "build_host", no_host_path)
+    with pytest.warns(RuntimeWarning, match="without their compiled host path"):
+        assert operators.require_device(torch.device("cuda", 0)) == 0
+    assert operators.fast is None and operators.require_device(torch.device("cuda", 0)) == 0      # said once

@@ -12,6 +12,7 @@ import importlib.util
 import subprocess
 import sysconfig
 import threading
+import warnings
 from pathlib import Path
 
 import torch
@@ -110,9 +111,19 @@ def host():
         if _host is None:
             library()                           # resident first: the host path links against it
             spec = importlib.util.spec_from_file_location("_ops_host", build_host())
-            _host = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(_host)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _host = module
         return _host
+
+
+def host_or_none():
+    """The host path, or None with a warning where it cannot be had: it saves microseconds a call, and every operator runs without it."""
+    try:
+        return host()
+    except (RuntimeError, OSError, ImportError) as error:
+        warnings.warn(f"trainkernel: the operators run without their compiled host path: {error}", RuntimeWarning, stacklevel=3)
+        return None
 
 
 def library() -> ctypes.CDLL:
@@ -158,9 +169,9 @@ def require_device(device: torch.device) -> int:
     if index not in _usable:
         capability = torch.cuda.get_device_capability(index)
         _usable[index] = capability[0] == 10
-        if _usable[index]:
-            host().allow_device(index)
-            fast = host()
+        if _usable[index] and (path := host_or_none()) is not None:
+            path.allow_device(index)
+            fast = path
     if not _usable[index]:
         raise RuntimeError("trainkernel: an sm_100 (B200-class) GPU is required")
     return index
