@@ -1,0 +1,96 @@
+"""The language-model operators at the edges of their ranges: large logits, tangents, layouts, overlaps, errors.
+
+Bounds are those of test_token_losses.py, derived there, unless a test says otherwise.
+"""
+import math
+
+import pytest
+import torch
+
+import trainkernel_b200 as tk
+from tests.test_token_losses import BF16, F16, F32, U, assert_grad, assert_logprobs, exact_preference, noise
+
+gpu = pytest.mark.gpu
+
+
+# -- rows whose largest logit is far from zero ---------------------------------------------------------------------
+
+TOPS = [-1e5, -1e8, -1e9, -1e10, -1e20, -1e30, 1e5, 1e8, 1e10, 1e20, 1e30]
+
+
+def far_rows(vocab, dtype, tops=TOPS):
+    """Per top: a uniform row, a row that mixes it with its neighbours below, and one with a few of it among zeros or lower ones."""
+    rows, targets = [], []
+    place = torch.arange(vocab, device="cuda")
+    for top in tops:
+        value = torch.full((vocab,), top, dtype=dtype, device="cuda")
+        below = value.float() - value.abs().float() * torch.finfo(dtype).eps * (place % 3)
+        rest = torch.where(place % 97 == 5, value.float(), min(4.0 * top, 0.0))
+        rows += [value, below.to(dtype), rest.to(dtype)]
+        targets += [vocab // 2, vocab - vocab % 3 - 3, vocab // 97 // 2 * 97 + 5]
+    return torch.stack(rows), torch.tensor(targets, device="cuda")
+
+
+def crossing_rows(vocab, scale):
+    """FP32 rows that pass from one side of +-2^16 to the other: up, down, by turns, and in runs of a vector, a block, a cluster's share."""
+    place = torch.arange(vocab, device="cuda", dtype=torch.float64)
+    forms = [place / vocab * 12 - 6, 6 - place / vocab * 12, (place % 2) * 3 - 1.5, (place // 4 % 2) * 3 - 1.5, (place // 1024 % 2) * 5 - 2.5, (place // (vocab / 8) % 2) * 5 - 2.5]
+    rows = torch.stack([sign * 65536.0 + form * scale for sign in (1, -1) for form in forms]).float()
+    return rows, torch.arange(len(rows), device="cuda") * (vocab // 13) + 1
+
+
+# (vocab, repeats): few rows of a short and a long vocabulary (rows split over blocks), many rows of every block shape
+PLACES = [(101, 1), (1003, 1), (1003, 60), (40001, 1), (20011, 40), (70001, 40)]
+
+
+def check_rows(rows, targets):
+    weights = noise((len(rows),), 1.0, 1)
+    assert_logprobs(tk.token_logprobs(rows, targets), rows, targets)
+    logp, grad = tk.token_logprobs_and_grad(rows, targets, weights)
+    assert_logprobs(logp, rows, targets)
+    assert_grad(grad, rows, targets, weights.double(), 2 * U)
+    leaf = rows.clone().requires_grad_()                       # statistics saved by one kernel, the gradient from them by another
+    (tk.token_logprobs(leaf, targets) * weights).sum().backward()
+    assert_grad(leaf.grad, rows, targets, weights.double(), 2 * U)
+
+
+@gpu
+@pytest.mark.parametrize("vocab,times", PLACES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_of_large_logits(vocab, times, dtype):
+    rows, targets = far_rows(vocab, dtype, TOPS if times == 1 or vocab < 20000 else TOPS[1::3])
+    check_rows(rows.repeat(times, 1)[:1000], targets.repeat(times)[:1000])
+
+
+@gpu
+@pytest.mark.parametrize("vocab,times", PLACES)
+@pytest.mark.parametrize("scale", [1.0, 1 / 16])
+def test_rows_on_both_sides_of_the_switch(vocab, times, scale):
+    rows, targets = crossing_rows(vocab, scale)
+    check_rows(rows.repeat(times, 1)[:720], targets.repeat(times)[:720])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_losses_of_rows_filled_with_a_large_negative_number(dtype):
+    """Every choice excluded with a finite constant: the tokens are uniform, and losses and gradients are numbers."""
+    vocab = 515
+    logits = noise((4, 3, vocab), 1.0, 2).to(dtype)
+    logits[:, 1] = -1e10
+    logits[2, 2] = -1e30
+    targets = torch.randint(0, vocab, (4, 3), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    logp = tk.token_logprobs(logits, targets)
+    assert_logprobs(logp, logits, targets)
+    old, advantages = logp.clone(), noise((4, 1), 1.0, 4)
+    loss, _, grad = tk.policy_loss_and_grad(logits, targets, old, advantages)
+    # the ratio is 1 up to two log-probabilities, each good to 60 u (its row is about 6 deep and has 515 logits)
+    assert abs(float(loss) + float(advantages.mean())) <= 128 * U * float(advantages.abs().max())
+    assert_grad(grad, logits, targets, (-advantages.double() / 12).expand(4, 3), 128 * U)
+    reference = noise((4,), 2.0, 5)
+    loss, sums, grad = tk.preference_loss_and_grad(logits, targets, reference, beta=0.5)
+    want, want_sums, slope = exact_preference(logits, targets, reference, None, 0.5, 0.0)
+    # three log-probabilities near -8 are added, each good to 64 u; z is off by half of four such sums, its sigmoid by a quarter of that
+    assert bool(((sums.double() - want_sums).abs() <= 3 * 64 * U + want_sums.abs() * U).all())
+    assert abs(float(loss) - float(want)) <= 0.5 * 4 * 192 * U + 16 * U * (1 + abs(float(want)))
+    relative = 0.5 * 4 * 192 * U + 16 * U                     # d log sigmoid' = 1 - sigmoid <= 1
+    assert_grad(grad, logits, targets, slope[:, None].expand(4, 3), relative)

@@ -21,7 +21,7 @@ using tk_ops::fail;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kExtreme = 1e38f;                  // beyond it logit * log2(e) may leave FP32's range
+constexpr float kExtreme = 65536.f;                // beyond it the rounding of logit * log2(e) is no longer small (see Exponent)
 
 // 2^x by the hardware's approximation (relative error about 2^-22).
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -129,8 +129,10 @@ __device__ __forceinline__ float scaled(float x) {
 }
 
 // The exponent of 2 that stands for exp(x - top): x log2(e) - rn(top log2(e)) in one fused operation.  The rounding of
-// the subtrahend is the same for every logit of the row and for its target, so it cancels.  Where the product could
-// overflow (logits of the type's lowest value everywhere) the difference is taken first.
+// the subtrahend is the same for every logit of the row and for its target, so it cancels, as long as 2 to that rounding
+// is an ordinary number: it is at most 2^-8 while |top| <= 2^16, which holds for all of FP16, and would reach 2^7 near 3e9,
+// where every term of the sum is infinite or zero.  Beyond 2^16 (rows filled with a large negative number in place of
+// -inf) the difference is taken first, which is exact to half a step and multiplied after.
 struct Exponent {
     float top, base;
     bool extreme;
@@ -142,13 +144,18 @@ struct Stat {
     float top, sum;                        // sum of 2^Exponent(top)(x)
 };
 
+// The exponent of 2 that takes a sum relative to the top `from` to one relative to `to`.  A sum is relative to its top's
+// rounded base, or, beyond kExtreme, to the product itself; what is subtracted is rounded as it was used.
+__device__ __forceinline__ float shift(float from, const Exponent& to) {
+    const bool far = fabsf(from) > kExtreme;
+    if (to.extreme) return far ? (from - to.top) * kLog2e : fmaf(-to.top, kLog2e, scaled(from));
+    return far ? fmaf(from, kLog2e, -to.base) : scaled(from) - to.base;
+}
+
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float top = fmaxf(a.top, b.top);
     const Exponent e(top);
-    // A part's sum is relative to its own rounded base, so the bases are what is subtracted, each rounded as it was used.
-    const float x = e.extreme ? (a.top - top) * kLog2e : scaled(a.top) - e.base;
-    const float y = e.extreme ? (b.top - top) * kLog2e : scaled(b.top) - e.base;
-    return {top, a.sum * exp2_fast(x) + b.sum * exp2_fast(y)};
+    return {top, a.sum * exp2_fast(shift(a.top, e)) + b.sum * exp2_fast(shift(b.top, e))};
 }
 
 // 2^(x log2(e) - base) with the exponent split at a whole number, so that its fraction keeps all of its bits: the rounding of
@@ -169,7 +176,7 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
     for (int i = 0; i < N; ++i) top = fmaxf(top, Vector<T>::top(v[i]));
     const Exponent e(top);
     if (!e.extreme) {
-        s.sum *= exp2_fast(scaled(s.top) - e.base);        // as in join; 0 while nothing was added
+        s.sum *= exp2_fast(shift(s.top, e));               // 0 while nothing was added
         s.top = top;
         const Pair scale = pair(kLog2e, kLog2e), base = pair(-e.base, -e.base);
         Pair sum = pair(0.f, 0.f);
