@@ -217,6 +217,9 @@ class SegmentedProgram:
                 else:
                     first = step.results[0]
                     operands = [self._window(values[value.buffer], value) for value in first.inputs]
+                    # The trace checked its own strides; here a value may lie in another order, and a kernel reads a row as one run.
+                    if operands[0].shape[-1] != 1 and operands[0].stride(-1) != 1:
+                        operands[0] = operands[0].contiguous()
                     arguments = [operands[value] if kind == "operand" else value for kind, value in first.attrs["arguments"]]
                     with torch.cuda.device(self.device):
                         results = IMPLEMENTATIONS[step.op](*arguments)
