@@ -192,6 +192,12 @@ class SegmentedProgram:
         return root if tuple(root.shape) == spec.shape and tuple(root.stride()) == spec.strides and spec.offset == 0 else \
             torch.as_strided(root, spec.shape, spec.strides, root.storage_offset() + spec.offset)
 
+    @staticmethod
+    def _dense(result: torch.Tensor) -> torch.Tensor:
+        """An operator's result as the next generated kernel takes it: a gradient may have its logits' strides, and lie like them within 16 bytes."""
+        result = result.contiguous()
+        return result.clone() if result.data_ptr() % 16 else result
+
     def __call__(self, *inputs: torch.Tensor) -> tuple[torch.Tensor, ...]:
         self._validate_inputs(inputs)
         for index in self.inplace_outputs.values():
@@ -225,7 +231,7 @@ class SegmentedProgram:
                         results = IMPLEMENTATIONS[step.op](*arguments)
                     results = (results,) if isinstance(results, torch.Tensor) else results
                     for op in step.results:
-                        values[op.output.buffer] = results[op.attrs["result"]].contiguous()      # a gradient may have its logits' strides
+                        values[op.output.buffer] = self._dense(results[op.attrs["result"]])
                 for buffer in self._frees[index]:
                     values.pop(buffer, None)
             for slot, spec in enumerate(self.program.outputs):
