@@ -6,7 +6,8 @@ import torch
 
 import trainkernel_b200 as tk
 from oracle import interpreter
-from trainkernel_b200 import segments
+from trainkernel_b200 import codegen, segments
+from trainkernel_b200.passes import fuse_loss_gradients
 
 gpu = pytest.mark.gpu
 IDS = torch.tensor([3, 0, 6, 2, 5])
@@ -108,3 +109,39 @@ def test_logits_at_an_odd_offset_and_the_product_behind_them():
     hot = torch.zeros(64, 128, device="cuda").scatter_(1, ids[:, None], 1.0)
     want = h.float().t() @ (hot - torch.softmax(x.float(), -1)).to(torch.bfloat16).float()
     assert float((got.float() - want).norm() / want.norm()) <= 2e-2
+
+
+# -- segments that read nothing ----------------------------------------------------------------------------------
+
+def summed(ids, logits):
+    return torch.func.grad(lambda x: -tk.token_logprobs(x, ids).sum())(logits)
+
+
+def averaged(ids, logits):
+    return torch.func.grad_and_value(lambda x: -tk.token_logprobs(x, ids).mean())(logits)
+
+
+@pytest.mark.parametrize("fn", [summed, averaged])
+def test_every_segment_has_an_input(fn):
+    """What flows back into the log-probabilities is a constant here: the kernel that writes it reads no tensor."""
+    inputs = (IDS, torch.randn(5, 7))
+    program, _ = tk.capture(fn, inputs)
+    steps, _ = segments.split_at_operators(fuse_loss_gradients(program))
+    parts = [step for step in steps if isinstance(step, segments.Segment)]
+    assert parts and all(part.program.inputs for part in parts)
+    for part in parts:
+        assert part.program.inputs[0].dtype == "float32"
+        codegen.generate(part.program)
+
+
+@gpu
+@pytest.mark.parametrize("fn", [summed, averaged])
+def test_the_gradient_of_a_cross_entropy_alone(fn):
+    ids, logits = IDS.cuda(), torch.randn(5, 7, device="cuda")
+    got, scale = tk.compile(fn, (ids, logits))(ids, logits), 1.0
+    if fn is averaged:
+        got, value = got
+        scale = 0.2
+        torch.testing.assert_close(value, -torch.log_softmax(logits, -1).gather(1, ids[:, None]).mean(), rtol=1e-5, atol=1e-5)
+    hot = torch.zeros_like(logits).scatter_(1, ids[:, None], 1.0)
+    torch.testing.assert_close(got, (torch.softmax(logits, -1) - hot) * scale, rtol=1e-5, atol=1e-6)

@@ -126,6 +126,8 @@ def split_at_operators(program: Program, inplace_outputs: dict[int, int] | None 
                 outputs.append(TensorSpec(buffer, op.output.shape, op.output.dtype, op.output.strides, buffer))
                 slots.append(("value", buffer))
         if outputs:
+            if not reads:                                        # constants only: a kernel takes at least one tensor
+                reads[next((spec for spec in program.inputs if spec.dtype.startswith(("float", "bfloat"))), program.inputs[0]).buffer] = None
             inputs = tuple(TensorSpec(b, roots[b].shape, roots[b].dtype, roots[b].strides, b) for b in reads)
             position = {spec.buffer: i for i, spec in enumerate(inputs)}
             steps.append(Segment(Program(inputs, tuple(ops), tuple(outputs)), tuple(slots), {k: position[b] for k, b in inplace.items()}))
