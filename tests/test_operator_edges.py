@@ -94,3 +94,51 @@ def test_losses_of_rows_filled_with_a_large_negative_number(dtype):
     assert abs(float(loss) - float(want)) <= 0.5 * 4 * 192 * U + 16 * U * (1 + abs(float(want)))
     relative = 0.5 * 4 * 192 * U + 16 * U                     # d log sigmoid' = 1 - sigmoid <= 1
     assert_grad(grad, logits, targets, slope[:, None].expand(4, 3), relative)
+
+
+# -- forward-mode derivatives --------------------------------------------------------------------------------------
+
+ON = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+
+
+def calls(logits, targets, old, reference):
+    """Every operator on the given tensors: name -> (call of the logits, call of one constant or None)."""
+    one = torch.ones((), device=logits.device)
+    return {
+        "token_logprobs": (lambda x: tk.token_logprobs(x, targets), None),
+        "token_logprobs_and_grad": (lambda x: tk.token_logprobs_and_grad(x, targets, old), lambda c: tk.token_logprobs_and_grad(logits, targets, c)),
+        "policy_loss": (lambda x: tk.policy_loss(x, targets, old, old), lambda c: tk.policy_loss(logits, targets, old, c)),
+        "policy_loss_and_grad": (lambda x: tk.policy_loss_and_grad(x, targets, old, old), lambda c: tk.policy_loss_and_grad(logits, targets, c, old)),
+        "policy_loss ref": (lambda x: tk.policy_loss(x, targets, old, old, ref_logprobs=old, kl_weight=0.1),
+                            lambda c: tk.policy_loss(logits, targets, old, old, ref_logprobs=c, kl_weight=0.1)),
+        "preference_loss": (lambda x: tk.preference_loss(x, targets, reference), lambda c: tk.preference_loss(logits, targets, c.sum(1))),
+        "preference_loss_and_grad": (lambda x: tk.preference_loss_and_grad(x, targets, reference), lambda c: tk.preference_loss_and_grad(logits, targets, c.sum(1))),
+        "grad_scale": (lambda x: tk.policy_loss_and_grad(x, targets, old, old, grad_scale=one),
+                       lambda c: tk.policy_loss_and_grad(logits, targets, old, old, grad_scale=c.sum())),
+    }
+
+
+@ON
+@pytest.mark.parametrize("name", calls(*[torch.zeros(1)] * 4))
+def test_forward_mode_is_refused_everywhere(device, name):
+    """A dropped tangent would read as a derivative of zero."""
+    from torch.autograd import forward_ad
+    logits, targets, old = torch.randn(2, 3, 5, device=device), torch.zeros((2, 3), dtype=torch.int64, device=device), torch.zeros((2, 3), device=device)
+    of_logits, of_constant = calls(logits, targets, old, old.sum(1))[name]
+    if device == "cuda":
+        of_logits(logits)                                      # from here on the compiled host path is asked first
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            of_logits(forward_ad.make_dual(logits, torch.ones_like(logits)))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            of_logits(forward_ad.make_dual(logits, torch.ones_like(logits))[:, :, :4])             # a view carries its tangent
+        if of_constant is not None:
+            with pytest.raises(ValueError, match="detach"):
+                of_constant(forward_ad.make_dual(old, torch.ones_like(old)))
+        if device == "cuda":
+            of_logits(logits)                                  # nothing else changes inside the level
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(of_logits, (logits,), (torch.ones_like(logits),))
+    if of_constant is not None:
+        with pytest.raises(ValueError, match="detach"):
+            torch.func.jvp(of_constant, (old,), (torch.ones_like(old),))

@@ -27,7 +27,8 @@ bool plain(PyObject* object) {
     using Key = c10::DispatchKey;
     static const c10::DispatchKeySet special({Key::Python, Key::PythonTLSSnapshot, Key::FuncTorchBatched, Key::FuncTorchGradWrapper, Key::Batched,
                                               Key::Functionalize, Key::Conjugate, Key::Negative, Key::ZeroTensor});
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_nested() && !t.key_set().has_any(special);
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_nested() || t.key_set().has_any(special)) return false;
+    return !t._fw_grad(0).defined();                           // a tangent is refused there
 }
 
 bool tracing() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }

@@ -5,7 +5,7 @@ Three operators, each in two forms:
 * `token_logprobs`, `policy_loss`, `preference_loss` are differentiable in the logits: by `torch.func`
   transforms inside a step handed to `compile` / `compile_training` (where the call becomes an IR
   operation that runs between two generated kernels), by the same transforms in eager code, and by
-  eager autograd.
+  eager autograd; once, and in reverse mode only (forward-mode derivatives are refused).
 * `token_logprobs_and_grad`, `policy_loss_and_grad`, `preference_loss_and_grad` return the gradient of
   the logits with the value, in the style of a compiled step.  They record no autograd history, read
   every logit from memory once where the mathematics allows it, and may be captured into a CUDA graph.
@@ -23,6 +23,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import operators
 from .operators import PolicyTerms, TokenArray, TokenGrad, TokenRows
@@ -35,6 +36,18 @@ _NO_ARRAY = (None, 0, 0)
 # ---------------------------------------------------------------------------
 # argument checks (metadata only: they hold for fake tensors too)
 # ---------------------------------------------------------------------------
+
+def _has_tangent(value: torch.Tensor) -> bool:
+    """Whether a forward-mode derivative travels with the tensor (`forward_ad.make_dual`, `torch.func.jvp`)."""
+    if forward_ad._current_level < 0:
+        return False
+    while True:
+        if not torch._C._functorch.is_batchedtensor(value) and forward_ad.unpack_dual(value).tangent is not None:
+            return True
+        if not torch._C._functorch.is_functorch_wrapped_tensor(value):
+            return False
+        value = torch._C._functorch.get_unwrapped(value)
+
 
 def _check_rows(who: str, logits, targets, mask, *, pairs: bool = False) -> None:
     if not isinstance(logits, torch.Tensor) or not isinstance(targets, torch.Tensor):
@@ -65,6 +78,8 @@ def _check_rows(who: str, logits, targets, mask, *, pairs: bool = False) -> None
             raise ValueError(f"trainkernel: {who}: inputs must use one device")
     if logits.is_neg() or logits.is_conj():
         raise ValueError("trainkernel: resolve lazy negative or conjugate input views before execution")
+    if _has_tangent(logits):
+        raise RuntimeError(f"trainkernel: {who} has no forward-mode derivative")
 
 
 def _check_constant(who: str, name: str, value, shape, device) -> torch.Tensor:
@@ -75,7 +90,7 @@ def _check_constant(who: str, name: str, value, shape, device) -> torch.Tensor:
         raise ValueError(f"trainkernel: {who}: {name} must be float32")
     if value.device != device:
         raise ValueError(f"trainkernel: {who}: inputs must use one device")
-    if value.requires_grad:
+    if value.requires_grad or _has_tangent(value):
         raise ValueError(f"trainkernel: {who}: no gradient flows to {name}; detach it")
     if value.is_neg():
         raise ValueError("trainkernel: resolve lazy negative or conjugate input views before execution")
@@ -97,6 +112,8 @@ def _check_scale(who: str, scale, device) -> tuple[float, torch.Tensor | None]:
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.numel() != 1 or scale.device != device:
             raise ValueError(f"trainkernel: {who}: a tensor grad_scale must hold one float32 value on the logits' device")
+        if _has_tangent(scale):
+            raise ValueError(f"trainkernel: {who}: no gradient flows to grad_scale; detach it")
         return 1.0, scale
     if isinstance(scale, bool) or not isinstance(scale, (int, float)):
         raise ValueError(f"trainkernel: {who}: grad_scale must be a number or a tensor of one float32 value")
