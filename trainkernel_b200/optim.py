@@ -13,7 +13,7 @@ from dataclasses import dataclass
 from typing import Any, Sequence
 
 import torch
-from torch.utils._pytree import tree_flatten
+from torch.utils._pytree import keystr, tree_flatten, tree_flatten_with_path
 
 from . import operators
 from .operators import AdamWOptions, AdamWTensor
@@ -29,11 +29,13 @@ class AdamWState:
     `offsets[i] + sizes[i]` in its own memory order, and offsets are multiples of 256.  With 32 bits
     `exp_avg` and `exp_avg_sq` are FP32.  With 8 bits `exp_avg` and `exp_avg_root` (the square root of
     the second moment) are e4m3 numbers that stand for themselves times the FP32 scale of their block
-    of 256, `exp_avg_scale` and `exp_avg_root_scale`.
+    of 256, `exp_avg_scale` and `exp_avg_root_scale`.  `paths` names the tensors by their place in the tree that
+    `init` was given (None for a plain list).
     """
 
-    def __init__(self, sizes: Sequence[int], bits: int, device: torch.device) -> None:
+    def __init__(self, sizes: Sequence[int], bits: int, device: torch.device, paths: Sequence[str] | None = None) -> None:
         self.sizes = tuple(sizes)
+        self.paths = None if paths is None else tuple(paths)
         self.bits = bits
         self.device = device
         offsets, total = [], 0
@@ -78,12 +80,13 @@ class AdamWState:
 
     def state_dict(self) -> dict[str, Any]:
         """Copies of the moments with the sizes they belong to, for a checkpoint."""
-        return {"sizes": self.sizes, "bits": self.bits, "tensors": tuple(t.clone() for t in self.tensors())}
+        return {"sizes": self.sizes, "bits": self.bits, "paths": self.paths, "tensors": tuple(t.clone() for t in self.tensors())}
 
     def load_state_dict(self, saved: dict[str, Any]) -> None:
         """Take over what `state_dict` of a state of the same sizes and bits returned."""
         if tuple(saved["sizes"]) != self.sizes or saved["bits"] != self.bits:
             raise ValueError("trainkernel: AdamW: the saved state belongs to other tensors or another number of bits")
+        _check_places("the saved state", _names(saved.get("paths")), "the state", self.paths)
         for mine, theirs in zip(self.tensors(), saved["tensors"]):
             mine.copy_(theirs)
 
@@ -105,6 +108,23 @@ def _leaves(tree: Any, what: str) -> list[torch.Tensor]:
     if not leaves or not all(isinstance(leaf, torch.Tensor) for leaf in leaves):
         raise TypeError(f"trainkernel: {what} must contain tensors only and cannot be empty")
     return leaves
+
+
+def _paths(tree: Any) -> tuple[str, ...] | None:
+    """Where every tensor of a tree stands; None for a tensor or a plain list or tuple of them, which go by position alone."""
+    if isinstance(tree, torch.Tensor) or isinstance(tree, (list, tuple)) and all(isinstance(x, torch.Tensor) for x in tree):
+        return None
+    return tuple(keystr(path) for path, _ in tree_flatten_with_path(tree)[0])
+
+
+def _names(paths: Any) -> tuple[str, ...] | None:
+    return None if paths is None else tuple(paths)
+
+
+def _check_places(what: str, paths: tuple[str, ...] | None, other: str, expected: tuple[str, ...] | None) -> None:
+    """Tensors are paired by position, and a dictionary has the order in which its keys were set: equal shapes would hide a mix-up."""
+    if paths is not None and expected is not None and paths != expected:
+        raise ValueError(f"trainkernel: AdamW: {what} must have the structure of {other}, dictionary keys in the same order")
 
 
 def _dense(tensor: torch.Tensor) -> bool:
@@ -181,7 +201,7 @@ class AdamW:
             self._check_param(leaf, device)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("trainkernel: AdamW: init inside a stream capture would clear the moments in every replay")
-        return AdamWState([leaf.numel() for leaf in leaves], self.state_bits, device)
+        return AdamWState([leaf.numel() for leaf in leaves], self.state_bits, device, _paths(params))
 
     @staticmethod
     def _check_param(leaf: torch.Tensor, device: torch.device) -> None:
@@ -197,6 +217,7 @@ class AdamW:
     def update(self, params: Any, grads: Any, state: AdamWState, *, grad_scale: torch.Tensor | None = None) -> None:
         """One step, in place, on the current stream.
 
+        `params` and `grads` are trees of the structure that `init` was given, or plain lists in the order of its leaves.
         `grads` matches `params` in shape and memory order (FP32, FP16 or BF16); parameters do not overlap.  `grad_scale` (one FP32 value on the
         device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
         not happen: parameters, moments and step count stay as they are.
@@ -211,6 +232,9 @@ class AdamW:
             raise ValueError(f"trainkernel: AdamW: the state holds {state.bits}-bit moments, this optimizer {self.state_bits}-bit ones")
         if len(leaves) != len(state.sizes) or len(gradients) != len(leaves):
             raise ValueError(f"trainkernel: AdamW: {len(leaves)} params and {len(gradients)} grads for a state of {len(state.sizes)} tensors")
+        places = _paths(params)
+        _check_places("params", places, "the tree that init was given", state.paths)
+        _check_places("grads", _paths(grads), "params", places if places is not None else state.paths)
         decays = self._decays(len(leaves))
         groups: dict[tuple, list] = {}
         storages = set()
