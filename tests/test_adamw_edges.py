@@ -67,3 +67,63 @@ def test_a_tree_is_updated_by_its_names():
     with pytest.raises(ValueError, match="same order"):
         optimizer.update({"layer": dict(reversed(params["layer"].items())), "head": params["head"]}, grads, state)
     assert int(state.step) == 1
+
+
+# -- tensors that share memory (a race inside the launch: refused before it) --------------------------------------
+
+ON = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+
+
+def flat(count, device):
+    return torch.zeros(count, device=device)
+
+
+@ON
+def test_overlapping_tensors_are_refused(device):
+    whole, apart = flat(1000, device), flat(1000, device)
+    number = flat(1, device)
+    optimizer = tk.AdamW()
+    if device == "cuda":
+        optimizer.update([number], [apart[:1]], optimizer.init([number]))        # the compiled host path is asked first from here on
+    cases = [
+        ([whole[:300], whole[299:400]], [apart[:300], apart[:101]], None, "params 0 and 1 overlap"),
+        ([whole[299:400], apart[:7], whole[:300]], [apart[10:111], apart[200:207], apart[300:600]], None, "overlap"),
+        ([whole[100:110], whole[:300]], [apart[:10], apart[10:310]], None, "overlap"),
+        ([whole[:300], whole[:300]], [apart[:300], apart[300:600]], None, "listed twice"),
+        ([whole[:300]], [whole[1:301]], None, "grad 0 overlaps param 0"),
+        ([whole[:300], apart[:5]], [apart[10:310], whole[295:300]], None, "grad 1 overlaps param 0"),
+        ([whole[:256], whole[256:512]], [whole[256:512], whole[:256]], None, "overlaps param"),
+        ([whole[:4].bfloat16().float()[:2], whole[:300]], [apart[:2], apart[:300]], whole[7:8], "grad_scale overlaps"),
+    ]
+    for params, grads, scale, message in cases:
+        with pytest.raises(ValueError, match=message):
+            optimizer.update(params, grads, state_of(params), grad_scale=scale)
+    assert not bool(whole.any())
+
+
+@ON
+def test_neighbours_and_a_gradient_in_its_own_param_are_accepted(device):
+    whole, apart = flat(1000, device) + 1.0, flat(1000, device) + 1.0
+    optimizer = tk.AdamW(lr=0.5, weight_decay=0.0)
+    cases = [([whole[:300], whole[300:301], whole[301:301], whole[301:1000]], [apart[:300], apart[300:301], apart[301:301], apart[301:1000]]),
+             ([whole[:300], whole[300:600]], [whole[:300], whole[600:900]])]
+    for params, grads in cases:
+        if device == "cpu":
+            with pytest.raises(RuntimeError, match="sm_100a GPU required"):
+                optimizer.update(params, grads, state_of(params))
+            continue
+        whole.fill_(1.0)
+        optimizer.update(params, grads, optimizer.init(params))
+        torch.testing.assert_close(whole[:600], torch.full((600,), 0.5, device=device), rtol=1e-5, atol=0.0)
+
+
+@gpu
+def test_the_short_way_leaves_overlaps_to_the_long_one():
+    from trainkernel_b200 import operators
+    whole, apart = flat(1000, "cuda"), flat(1000, "cuda")
+    optimizer = tk.AdamW()
+    for params, grads, taken in (([whole[:300], whole[300:600]], [apart[:300], apart[300:600]], True), ([whole[:300], whole[299:600]], [apart[:300], apart[300:601]], False),
+                                 ([whole[:300], apart[:5]], [apart[10:310], whole[295:300]], False)):
+        state = optimizer.init(params)
+        answer = operators.fast.adamw_update(params, grads, state.sizes, state.offsets, 0.0, state._struct_at, state._tensors, 32, 0.0, (0.9, 0.9), 1e-8, 0, None)
+        assert bool(answer) == taken

@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <iterator>
 #include <vector>
 
 #include "trainkernel_ops.h"
@@ -234,6 +235,22 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
     return true;
 }
 
+// Bytes of dense tensors, and whether one lies among others that are sorted and apart.
+struct Span {
+    uintptr_t begin, end;
+    bool operator<(const Span& other) const { return begin < other.begin; }
+};
+
+Span span_of(const at::Tensor& t) {
+    const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return {begin, begin + static_cast<uintptr_t>(t.numel()) * t.element_size()};
+}
+
+bool among(const std::vector<Span>& spans, const Span& s) {
+    const auto behind = std::lower_bound(spans.begin(), spans.end(), Span{s.end, 0});       // the first that begins at its end or later
+    return s.begin < s.end && behind != spans.begin() && std::prev(behind)->end > s.begin;
+}
+
 // (params, grads, sizes, offsets, decay, state struct address, state tensors, bits, lr, betas, eps, seed, grad_scale) -> True
 // Only for lists of contiguous tensors of one parameter type and one gradient type.
 PyObject* adamw_update(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -253,7 +270,7 @@ PyObject* adamw_update(PyObject*, PyObject* const* args, Py_ssize_t count) {
         options.bits = static_cast<int32_t>(bits);
         options.seed = static_cast<uint32_t>(seed);
         std::vector<tk_adamw_tensor> tensors(static_cast<size_t>(n));
-        std::vector<void*> places;
+        std::vector<Span> places, gradients;
         places.reserve(static_cast<size_t>(n));
         int param_type = -1, grad_type = -1;
         c10::Device device(c10::kCPU);
@@ -276,20 +293,23 @@ PyObject* adamw_update(PyObject*, PyObject* const* args, Py_ssize_t count) {
             double d = one_decay;
             if (PyTuple_CheckExact(decay) && !number(PyTuple_GET_ITEM(decay, i), &d)) Py_RETURN_NONE;
             tensors[i] = {p.data_ptr(), g.data_ptr(), PyLong_AsLongLong(PyTuple_GET_ITEM(offsets, i)), size, static_cast<float>(d), 0};
-            if (size) places.push_back(p.data_ptr());
+            if (size) places.push_back(span_of(p));
+            if (size && (g.data_ptr() != p.data_ptr() || grad_type != param_type)) gradients.push_back(span_of(g));      // its own param's memory is read before it is written
         }
         if (device.index() < 0 || device.index() >= 64 || !g_usable[device.index()]) Py_RETURN_NONE;
         std::sort(places.begin(), places.end());
-        if (std::adjacent_find(places.begin(), places.end()) != places.end()) Py_RETURN_NONE;
+        if (std::adjacent_find(places.begin(), places.end(), [](const Span& a, const Span& b) { return a.end > b.begin; }) != places.end()) Py_RETURN_NONE;
+        for (const Span& gradient : gradients)
+            if (among(places, gradient)) Py_RETURN_NONE;
         if (args[12] != Py_None) {
             if (!plain(args[12])) Py_RETURN_NONE;
             const at::Tensor& scale = THPVariable_Unpack(args[12]);
-            if (scale.scalar_type() != at::kFloat || scale.numel() != 1 || scale.device() != device) Py_RETURN_NONE;
+            if (scale.scalar_type() != at::kFloat || scale.numel() != 1 || scale.device() != device || among(places, span_of(scale))) Py_RETURN_NONE;
             options.scale_at = scale.data_ptr<float>();
         }
         if (!lr_given) {
             const at::Tensor& lr = THPVariable_Unpack(args[8]);
-            if (lr.scalar_type() != at::kFloat || lr.numel() != 1 || lr.device() != device) Py_RETURN_NONE;
+            if (lr.scalar_type() != at::kFloat || lr.numel() != 1 || lr.device() != device || among(places, span_of(lr))) Py_RETURN_NONE;
             options.lr_at = lr.data_ptr<float>();
         }
         for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[6]); ++i) {

@@ -8,6 +8,7 @@ runs it behind a compiled step.  The reference's only update is SGD inside the s
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 from dataclasses import dataclass
 from typing import Any, Sequence
@@ -139,6 +140,39 @@ def _dense(tensor: torch.Tensor) -> bool:
     return True
 
 
+def _span(tensor: torch.Tensor) -> tuple[int, int]:
+    """First byte of a dense tensor and the one behind its last."""
+    begin = tensor.data_ptr()
+    return begin, begin + tensor.numel() * tensor.element_size()
+
+
+def _check_apart(leaves: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor], values: dict[str, Any]) -> None:
+    """Nothing the launch writes may be written twice or read by another block: every param has memory of its own.  A
+    gradient may be its own param's memory, where each element is read before it is written."""
+    spans = sorted((*_span(leaf), i) for i, leaf in enumerate(leaves) if leaf.numel())
+    for (a, end, i), (b, _, j) in zip(spans, spans[1:]):
+        if a == b:
+            raise ValueError(f"trainkernel: AdamW: param {max(i, j)} is listed twice")
+        if b < end:
+            raise ValueError(f"trainkernel: AdamW: params {i} and {j} overlap in memory")
+
+    def over(tensor: torch.Tensor) -> int | None:
+        """The first param that a tensor overlaps."""
+        begin, end = _span(tensor)
+        at = bisect.bisect_left(spans, (begin,))
+        if at and spans[at - 1][1] > begin:
+            at -= 1
+        return spans[at][2] if at < len(spans) and spans[at][0] < end and spans[at][1] > begin else None
+
+    for i, grad in enumerate(gradients):
+        where = over(grad) if grad.numel() else None
+        if where is not None and not (where == i and grad.data_ptr() == leaves[i].data_ptr() and grad.dtype == leaves[i].dtype):
+            raise ValueError(f"trainkernel: AdamW: grad {i} overlaps param {where} in memory")
+    for name, value in values.items():
+        if isinstance(value, torch.Tensor) and over(value) is not None:
+            raise ValueError(f"trainkernel: AdamW: {name} overlaps a param in memory")
+
+
 def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
 
@@ -218,8 +252,8 @@ class AdamW:
         """One step, in place, on the current stream.
 
         `params` and `grads` are trees of the structure that `init` was given, or plain lists in the order of its leaves.
-        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16); parameters do not overlap.  `grad_scale` (one FP32 value on the
-        device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
+        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16).  No two params overlap in memory, and nothing else
+        overlaps one, but a gradient its own param.  `grad_scale` (one FP32 value on the device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
         not happen: parameters, moments and step count stay as they are.
         """
         if operators.fast is not None and state.bits == self.state_bits and operators.fast.adamw_update(
@@ -237,7 +271,6 @@ class AdamW:
         _check_places("grads", _paths(grads), "params", places if places is not None else state.paths)
         decays = self._decays(len(leaves))
         groups: dict[tuple, list] = {}
-        storages = set()
         for i, (leaf, grad) in enumerate(zip(leaves, gradients)):
             self._check_param(leaf, device)
             if leaf.numel() != state.sizes[i]:
@@ -246,17 +279,13 @@ class AdamW:
                 raise ValueError(f"trainkernel: AdamW: grad {i} does not match its param in shape, device or type")
             if not _same_order(leaf, grad):
                 raise ValueError(f"trainkernel: AdamW: grad {i} must have its param's memory order")
-            if leaf.numel():
-                at = leaf.data_ptr()
-                if at in storages:
-                    raise ValueError(f"trainkernel: AdamW: param {i} is listed twice")
-                storages.add(at)
             groups.setdefault((leaf.dtype, grad.dtype), []).append((leaf.data_ptr(), grad.data_ptr(), state.offsets[i], state.sizes[i], decays[i], 0))
         for name, value in (("lr", self.lr), ("grad_scale", grad_scale)):
             if isinstance(value, torch.Tensor) and (value.device != device or value.dtype != torch.float32 or value.numel() != 1):
                 raise ValueError(f"trainkernel: AdamW: a tensor {name} must hold one float32 value on the params' device")
         if grad_scale is not None and not isinstance(grad_scale, torch.Tensor):
             raise ValueError("trainkernel: AdamW: grad_scale must be a tensor of one float32 value")
+        _check_apart(leaves, gradients, {"lr": self.lr, "grad_scale": grad_scale})
         by_tensor = isinstance(self.lr, torch.Tensor)
         options = AdamWOptions(self.lr.data_ptr() if by_tensor else None, None if grad_scale is None else grad_scale.data_ptr(),
                                0.0 if by_tensor else self.lr, *self.betas, self.eps, self.seed, self.state_bits)
