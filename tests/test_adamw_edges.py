@@ -127,3 +127,19 @@ def test_the_short_way_leaves_overlaps_to_the_long_one():
         state = optimizer.init(params)
         answer = operators.fast.adamw_update(params, grads, state.sizes, state.offsets, 0.0, state._struct_at, state._tensors, 32, 0.0, (0.9, 0.9), 1e-8, 0, None)
         assert bool(answer) == taken
+
+
+@gpu
+def test_an_earlier_call_s_error_is_not_this_call_s():
+    """A call on a device that does not exist fails on the host; the update behind it is answered for itself."""
+    from trainkernel_b200 import operators
+    params, grads = [torch.ones(300, device="cuda")], [torch.ones(300, device="cuda")]
+    optimizer = tk.AdamW(lr=0.5, weight_decay=0.0)
+    state = optimizer.init(params)
+    logits, targets, out = torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(2, device="cuda")
+    rows = operators.TokenRows(logits.data_ptr(), 0, 8, 1, 2, 8, 0, 8, operators.TokenArray(targets.data_ptr(), 0, 1), operators.TokenArray())
+    lib = operators.library()
+    assert lib.tk_token_logprobs(rows, out.data_ptr(), None, 63, None) not in (0, 100001) and b"selecting the device" in lib.tk_ops_last_error()
+    optimizer.update(params, grads, state)
+    assert int(state.step) == 1
+    torch.testing.assert_close(params[0], torch.full((300,), 0.5, device="cuda"), rtol=1e-5, atol=0.0)

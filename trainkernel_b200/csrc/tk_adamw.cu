@@ -387,9 +387,12 @@ int launch(const tk_adamw_tensor* tensors, int count, const tk_adamw_state* stat
     if (grid > TK_ADAMW_COUNTERS) grid = TK_ADAMW_COUNTERS;
     if (grid > chunks) grid = chunks;
     if (grid < 1) grid = 1;
-    adamw_kernel<P, G, BITS, CAPACITY><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(grid));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
     count_launch();
-    return check(cudaGetLastError(), "launching the AdamW kernel");
+    return check(cudaLaunchKernelEx(&config, adamw_kernel<P, G, BITS, CAPACITY>, a), "launching the AdamW kernel");
 }
 
 template <typename P, typename G, int BITS>

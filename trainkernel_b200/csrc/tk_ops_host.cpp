@@ -23,6 +23,7 @@ int fail(int code, const char* format, ...) {
 
 int check(cudaError_t status, const char* what) {
     if (status == cudaSuccess) return 0;
+    cudaGetLastError();                            // reported here and now: it must not be taken for a later call's
     return fail(static_cast<int>(status), "trainkernel: %s failed: %s", what, cudaGetErrorString(status));
 }
 
