@@ -58,7 +58,7 @@ typedef struct {
 } tk_token_grad;
 
 typedef struct {
-    tk_token_array old_logprobs, advantages, ref_logprobs;   /* FP32; ref_logprobs.data may be NULL */
+    tk_token_array old_logprobs, advantages, ref_logprobs;   /* FP32; ref_logprobs.data may be NULL, and is not read when kl_weight is 0 */
     float clip_low, clip_high, kl_weight;
     int32_t average;                                         /* TK_AVERAGE_* */
 } tk_policy_terms;

@@ -94,7 +94,7 @@ def _policy(logits, targets, old, advantages, ref, mask, low, high, kl_weight, a
     ratio = torch.exp(logp - old.double())
     free, bound = ratio * advantages, ratio.clamp(1 - low, 1 + high) * advantages
     term, slope = -torch.minimum(free, bound), torch.where(free <= bound, -free, torch.zeros_like(free))
-    if ref is not None:
+    if ref is not None and kl_weight:
         away = ref.double() - logp
         term, slope = term + kl_weight * (torch.exp(away) - away - 1), slope + kl_weight * (1 - torch.exp(away))
     weight = keep.double()

@@ -142,3 +142,18 @@ def test_forward_mode_is_refused_everywhere(device, name):
     if of_constant is not None:
         with pytest.raises(ValueError, match="detach"):
             torch.func.jvp(of_constant, (old,), (torch.ones_like(old),))
+
+
+# -- terms of weight zero ------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_kl_term_of_weight_zero_is_no_term(grad):
+    """exp(ref - logprob) overflows FP32 from 89 on; its weight says that nothing of it is wanted."""
+    logits, targets = noise((2, 3, 50), 1.0, 6), torch.zeros((2, 3), dtype=torch.int64, device="cuda")
+    old = tk.token_logprobs(logits, targets)
+    form = tk.policy_loss_and_grad if grad else tk.policy_loss
+    want = form(logits, targets, old, torch.ones_like(old))
+    for ref in (old + 200.0, torch.full_like(old, float("inf")), torch.full_like(old, float("nan"))):
+        for a, b in zip(form(logits, targets, old, torch.ones_like(old), ref_logprobs=ref, kl_weight=0.0), want):
+            assert torch.equal(a, b)

@@ -820,6 +820,7 @@ extern "C" int tk_policy_loss(const tk_token_rows* rows, const tk_policy_terms* 
     if (scope.status) return scope.status;
     Args a = arguments(rows, grad);
     a.policy = *terms;
+    if (terms->kl_weight == 0.f) a.policy.ref_logprobs.data = nullptr;      // no term: 0 times an exponential that overflows is not 0
     a.logprobs = logprobs;
     a.stats = stats;
     a.row_coefficients = coefficients;

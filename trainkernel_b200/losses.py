@@ -488,7 +488,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
     Per counted token, with `r = exp(logprob - old_logprob)`:
     `-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_weight (exp(d) - d - 1)`, `d = ref_logprob - logprob`.
     `average="tokens"` averages over all counted tokens; `"sequences"` over the tokens of each sequence and then over
-    all `batch` sequences (one without counted tokens contributes 0).  With nothing counted the loss is 0.
+    all `batch` sequences (one without counted tokens contributes 0).  With nothing counted the loss is 0.  With a
+    `kl_weight` of 0 `ref_logprobs` is not read.
     """
     if operators.fast is not None and (done := operators.fast.policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip,
                                                                           kl_weight, average, None)) is not None:
