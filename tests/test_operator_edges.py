@@ -157,3 +157,18 @@ def test_a_kl_term_of_weight_zero_is_no_term(grad):
     for ref in (old + 200.0, torch.full_like(old, float("inf")), torch.full_like(old, float("nan"))):
         for a, b in zip(form(logits, targets, old, torch.ones_like(old), ref_logprobs=ref, kl_weight=0.0), want):
             assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("side", [0, 1])
+def test_a_token_of_probability_zero_decides_its_pair(side):
+    """With label_smoothing 0 a pair whose rejected sequence cannot occur has loss 0, one whose preferred sequence cannot has loss inf."""
+    logits, targets = noise((2, 3, 50), 1.0, 7), torch.zeros((2, 3), dtype=torch.int64, device="cuda")
+    logits[side, 1, 0] = -float("inf")
+    loss, sums, grad = tk.preference_loss_and_grad(logits, targets, torch.zeros(2, device="cuda"), beta=0.5)
+    assert float(sums[side]) == -float("inf") and bool(torch.isfinite(sums[1 - side])) and bool(torch.isfinite(grad).all())
+    assert float(loss) == (0.0 if side else float("inf"))
+    assert bool((grad == 0).all()) == bool(side)
+    # turned round by a smoothing of 1; with both terms, each infinite somewhere, the loss is infinite
+    assert float(tk.preference_loss(logits, targets, torch.zeros(2, device="cuda"), beta=0.5, label_smoothing=1.0)[0]) == (float("inf") if side else 0.0)
+    assert float(tk.preference_loss(logits, targets, torch.zeros(2, device="cuda"), beta=0.5, label_smoothing=0.5)[0]) == float("inf")

@@ -648,7 +648,8 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int64_t pairs, in
         const float z = static_cast<float>(beta * ((both[0] - reference[pair * reference_stride])
                                                    - (both[1] - reference[(pair + pairs) * reference_stride])));
         const float tail = log1pf(expf(-fabsf(z)));
-        const float term = (1.f - smoothing) * (fmaxf(-z, 0.f) + tail) + smoothing * (fmaxf(z, 0.f) + tail);
+        // A weight of 0 drops its term: z is infinite where one sequence has a token of probability 0.
+        const float term = (smoothing < 1.f ? (1.f - smoothing) * (fmaxf(-z, 0.f) + tail) : 0.f) + (smoothing > 0.f ? smoothing * (fmaxf(z, 0.f) + tail) : 0.f);
         const float up = 1.f / (1.f + expf(-z)), down = 1.f / (1.f + expf(z));
         const float slope = beta / static_cast<float>(pairs) * (smoothing * up - (1.f - smoothing) * down);
         // fmaxf drops NaN; a pair that has one must show it
