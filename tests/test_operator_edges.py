@@ -172,3 +172,41 @@ def test_a_token_of_probability_zero_decides_its_pair(side):
     # turned round by a smoothing of 1; with both terms, each infinite somewhere, the loss is infinite
     assert float(tk.preference_loss(logits, targets, torch.zeros(2, device="cuda"), beta=0.5, label_smoothing=1.0)[0]) == (float("inf") if side else 0.0)
     assert float(tk.preference_loss(logits, targets, torch.zeros(2, device="cuda"), beta=0.5, label_smoothing=0.5)[0]) == float("inf")
+
+
+# -- layouts -------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("form", ["policy_loss_and_grad", "preference_loss_and_grad", "token_logprobs_and_grad", "backward"])
+def test_a_trace_of_shifted_logits_meets_the_layout_that_it_saw(form):
+    """A graph traced with fake tensors, run on real ones: `view` on the gradient is only possible where it is as dense as declared."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    logits = noise((4, 6, 33), 1.0, 8).to(BF16)[:, :-1]
+    targets, old = torch.zeros((4, 5), dtype=torch.int64, device="cuda"), noise((4, 5), 0.1, 9) - 3.5
+
+    def gradient(x):
+        if form == "policy_loss_and_grad":
+            return tk.policy_loss_and_grad(x, targets, old, old)[2]
+        if form == "preference_loss_and_grad":
+            return tk.preference_loss_and_grad(x, targets, old[:, 0])[2]
+        if form == "token_logprobs_and_grad":
+            return tk.token_logprobs_and_grad(x, targets, old)[1]
+        return torch.func.grad(lambda y: (tk.token_logprobs(y, targets) * old).sum())(x)
+
+    graph = make_fx(lambda x: gradient(x).view(-1) * 1.0, tracing_mode="fake", _allow_non_fake_inputs=True)(logits)
+    got, want = graph(logits), gradient(logits)
+    assert torch.equal(got, want.reshape(-1))
+    assert want.stride() == logits.stride()                    # called directly, it lies as its logits do, without a copy
+
+
+@gpu
+def test_the_eager_gradient_of_shifted_logits_lies_as_they_do():
+    whole = noise((4, 6, 33), 1.0, 10).requires_grad_()
+    shifted = whole[:, :-1]
+    seen = []
+    shifted.register_hook(lambda grad: seen.append(grad.stride()))
+    targets = torch.zeros((4, 5), dtype=torch.int64, device="cuda")
+    tk.token_logprobs(shifted, targets).sum().backward()
+    assert seen == [shifted.stride()]
+    assert_grad(whole.grad[:, :-1], shifted.detach(), targets, torch.ones((4, 5), dtype=torch.float64, device="cuda"), 2 * U)
+    assert bool((whole.grad[:, -1] == 0).all())

@@ -324,8 +324,16 @@ def _no_cpu(*args):
     raise RuntimeError("trainkernel: CUDA sm_100a GPU required; CPU IR inspection is available through capture()")
 
 
+def _as_declared(run):
+    """What a traced call runs on real tensors: results as dense as `_SHAPES` says, which a trace relies on."""
+    def dense(*args):
+        results = run(*args)
+        return results.contiguous() if isinstance(results, torch.Tensor) else tuple(result.contiguous() for result in results)
+    return dense
+
+
 for _name, _run in IMPLEMENTATIONS.items():
-    _ops.impl(_name, _run, "CUDA")
+    _ops.impl(_name, _as_declared(_run), "CUDA")
     _ops.impl(_name, _no_cpu, "CPU")
     torch.library.register_fake(f"trainkernel::{_name}", _SHAPES[_name], lib=_ops)
 
@@ -341,6 +349,8 @@ class _LogitsGrad(torch.autograd.Function):
 
     @staticmethod
     def forward(logits, targets, mask, coefficients, stats, scale):
+        if logits.is_cuda and _is_plain(logits, targets, mask, coefficients, stats, scale):
+            return _logits_grad_launch(logits, targets, mask, coefficients, stats, scale)          # with the logits' strides
         return _call.token_logits_grad(logits, targets, mask, coefficients, stats, scale)
 
     @staticmethod
