@@ -210,3 +210,27 @@ def test_the_eager_gradient_of_shifted_logits_lies_as_they_do():
     assert seen == [shifted.stride()]
     assert_grad(whole.grad[:, :-1], shifted.detach(), targets, torch.ones((4, 5), dtype=torch.float64, device="cuda"), 2 * U)
     assert bool((whole.grad[:, -1] == 0).all())
+
+
+@gpu
+def test_a_tensor_subclass_goes_the_long_way():
+    """Its operations may mean something else, so the call is dispatched; the values are the same."""
+    from trainkernel_b200 import operators
+
+    class Marked(torch.Tensor):
+        seen = 0
+
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            cls.seen += "trainkernel" in str(func)
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    logits, targets = noise((3, 40), 1.0, 11), torch.zeros(3, dtype=torch.int64, device="cuda")
+    want = tk.token_logprobs(logits, targets)                  # from here on the compiled host path is asked first
+    marked = logits.as_subclass(Marked)
+    for arguments in ((marked, targets, None), (logits, targets.as_subclass(Marked), None), (logits, targets, (targets == 0).as_subclass(Marked))):
+        assert operators.fast.token_logprobs(*arguments) is None
+    assert operators.fast.token_logprobs(torch.nn.Parameter(logits, requires_grad=False), targets, None) is not None
+    logp, grad = tk.token_logprobs_and_grad(marked, targets, torch.ones(3, device="cuda"))
+    assert Marked.seen and torch.equal(logp.as_subclass(torch.Tensor), want)
+    assert torch.equal(tk.token_logprobs(marked, targets).as_subclass(torch.Tensor), want)

@@ -23,7 +23,7 @@ bool g_usable[64] = {};
 
 // Why a call goes the long way round is decided there, so all of these only say yes or no.
 bool plain(PyObject* object) {
-    if (!THPVariable_CheckExact(object) && !THPVariable_Check(object)) return false;
+    if (!THPVariable_CheckExact(object)) return false;         // a Tensor or a Parameter: a subclass may mean something else by its operations
     const at::Tensor& t = THPVariable_Unpack(object);
     using Key = c10::DispatchKey;
     static const c10::DispatchKeySet special({Key::Python, Key::PythonTLSSnapshot, Key::FuncTorchBatched, Key::FuncTorchGradWrapper, Key::Batched,
