@@ -725,15 +725,18 @@ int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
     while (shares < kMostShares && grid * shares * 2 <= sms && bytes / (shares * 2) >= 8 * 1024) shares *= 2;
     if (shares > 1) return launch_clusters(token_rows_kernel<T, MODE, LOSS, 256, 2, true>, grid * shares, shares, 256, 0, early, stream, a, 0);
     if (bytes <= 16 * 1024 && grid > 4 * sms) return launch(token_rows_kernel<T, MODE, LOSS, 96, 18, false>, grid, 96, 0, early, stream, a, 0);
-    if (MODE != kBoth && bytes > 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
-    if (bytes <= 80 * 1024 || !a.in_phase) return launch(token_rows_kernel<T, MODE, LOSS, 256, 6, false>, grid, 256, 0, early, stream, a, 0);
-    auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2, false>;
-    static std::atomic<bool> sized[64];
-    if (device >= 64 || !sized[device].load(std::memory_order_relaxed)) {
-        if (int code = check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptVectors * 16), "sizing shared memory")) return code;
-        if (device < 64) sized[device].store(true, std::memory_order_relaxed);
+    if constexpr (MODE != kBoth) {
+        if (bytes > 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
+    } else if (bytes > 80 * 1024 && a.in_phase) {
+        auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2, false>;
+        static std::atomic<bool> sized[64];
+        if (device >= 64 || !sized[device].load(std::memory_order_relaxed)) {
+            if (int code = check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptVectors * 16), "sizing shared memory")) return code;
+            if (device < 64) sized[device].store(true, std::memory_order_relaxed);
+        }
+        return launch(kernel, grid, 640, kKeptVectors * 16, early, stream, a, kKeptVectors);
     }
-    return launch(kernel, grid, 640, kKeptVectors * 16, early, stream, a, kKeptVectors);
+    return launch(token_rows_kernel<T, MODE, LOSS, 256, 6, false>, grid, 256, 0, early, stream, a, 0);
 }
 
 template <Mode MODE, Loss LOSS>

@@ -15,7 +15,7 @@ from typing import Any, Sequence
 
 import torch
 
-from .ir import Operation, Program, TensorSpec, row_major, validate
+from .ir import Operation, Program, TensorSpec, validate
 from .losses import IMPLEMENTATIONS
 from .passes import fuse_loss_gradients
 
@@ -49,10 +49,6 @@ class Segment:
 
 def _operands(op: Operation) -> list[TensorSpec]:
     return [value for value in op.inputs if isinstance(value, TensorSpec)]
-
-
-def _is_root(spec: TensorSpec) -> bool:
-    return spec.offset == 0 and spec.strides == row_major(spec.shape)
 
 
 def split_at_operators(program: Program, inplace_outputs: dict[int, int] | None = None) -> tuple[list[Segment | Call], dict[int, int]]:
@@ -148,7 +144,6 @@ class SegmentedProgram:
         self.inplace_outputs = dict(inplace_outputs)
         self.late = dict(late)
         self._input_meta = [(spec.shape, spec.strides, getattr(torch, spec.dtype)) for spec in program.inputs]
-        self._final = [step for step, _ in self.steps]
         # values are dropped behind their last reader, so a long program does not hold all of them
         self._frees: list[tuple[str, ...]] = []
         last: dict[str, int] = {}
