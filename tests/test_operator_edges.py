@@ -234,3 +234,30 @@ def test_a_tensor_subclass_goes_the_long_way():
     logp, grad = tk.token_logprobs_and_grad(marked, targets, torch.ones(3, device="cuda"))
     assert Marked.seen and torch.equal(logp.as_subclass(torch.Tensor), want)
     assert torch.equal(tk.token_logprobs(marked, targets).as_subclass(torch.Tensor), want)
+
+
+# -- many masked rows ----------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(5000, 333, BF16), (16384, 40, F32), (1000, 20011, F16), (1024, 50257, BF16), (3000, 9001, F32)])
+@pytest.mark.parametrize("counted", [1.0, 0.5, 0.01])
+def test_policy_loss_of_many_rows_without_a_batch(rows, vocab, dtype, counted):
+    """Rows that run at once, rows behind them and masked rows of both kinds; repeated, because their order is not fixed."""
+    logits = noise((rows, vocab), 2.0, 12).to(dtype)
+    targets = torch.randint(0, vocab, (rows,), generator=torch.Generator(device="cuda").manual_seed(13), device="cuda", dtype=torch.int32)
+    mask = torch.rand(rows, generator=torch.Generator(device="cuda").manual_seed(14), device="cuda") < counted
+    mask[0] = counted < 1                                      # the first row counts, or is the only one that does not
+    every = tk.token_logprobs(logits, targets)
+    old, advantages = every + noise((rows,), 0.1, 15), noise((rows,), 1.0, 16)
+    logp = torch.log_softmax(logits.double(), -1).gather(1, targets.long()[:, None])[:, 0]
+    ratio = torch.exp(logp - old)
+    terms = -torch.minimum(ratio * advantages, ratio.clamp(0.5, 2.0) * advantages)
+    want = float(terms[mask].mean())
+    # a log-probability is off by d, its ratio by that and 4 u relative; ratios are below 2
+    x = logits.double()
+    d = float(U * (4 * (x.amax(-1) - x.amin(-1)).max() + vocab / 256 + 40))
+    for _ in range(5):
+        loss, got, grad = tk.policy_loss_and_grad(logits, targets, old, advantages, mask=mask, clip=(0.5, 1.0))
+        assert torch.equal(got == 0, ~mask) and bool((grad[~mask] == 0).all()) and bool((grad[mask] != 0).any())
+        assert abs(float(loss) - want) <= 2 * float(advantages.abs().max()) * (d + 8 * U) + 4 * U * abs(want)
+        assert abs(float(tk.policy_loss(logits, targets, old, advantages, mask=mask, clip=(0.5, 1.0))[0]) - want) <= 2 * float(advantages.abs().max()) * (d + 8 * U) + 4 * U * abs(want)

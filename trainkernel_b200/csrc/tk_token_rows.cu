@@ -212,7 +212,6 @@ __device__ __forceinline__ void accumulate_one(Stat& s, T value) {
 }
 
 enum Mode { kStats, kGrad, kBoth };            // log-probabilities / gradient from saved stats / both
-constexpr int kFirstRows = 2048;               // more rows than blocks run at once
 
 enum Loss { kWeights, kPolicy };               // where kBoth takes the coefficient from, and what kStats adds
 
@@ -230,6 +229,7 @@ struct Args {
     float* weights;                            // one per sequence
     float* terms;                              // one per row
     float* loss;
+    int64_t first_rows;                        // rows whose blocks start at once; those behind them start when one has ended
     unsigned* clear;                           // a word block 0 zeroes for the kernel that follows, or NULL
 };
 
@@ -524,7 +524,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __gri
             advantage = at(a.policy.advantages, b, t);
             if (a.policy.ref_logprobs.data) ref_logprob = at(a.policy.ref_logprobs, b, t);
             // The first blocks start beside the kernel that computes the weights and ask for theirs behind the statistics.
-            if (row >= kFirstRows) {
+            // When a later one starts it has ended, and the wait costs nothing.
+            if (row >= a.first_rows) {
                 wait_for_previous();
                 weight = a.weights[b];
             }
@@ -545,9 +546,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __gri
         }
         if (LOSS == kPolicy) {
             float term = 0.f, slope = 0.f;
-            if (row < kFirstRows) wait_for_previous();
+            if (row < a.first_rows || !keep) wait_for_previous();              // for the counter too
             if (keep) {
-                if (row < kFirstRows) weight = a.weights[b];
+                if (row < a.first_rows) weight = a.weights[b];
                 policy_token(a.policy, old_logprob, advantage, ref_logprob, logprob, &term, &slope);
                 term *= weight;
                 slope *= weight;
@@ -717,16 +718,25 @@ constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
 // 158 us of those rows with 3 blocks of 512 threads, 161 with 6 of 256, 176 with 8 of 256.  Short rows that all run at once
 // get more threads each (256 x 1000 FP32 with gradient, captured: 7.0 us with 256, 7.2 with 128, 8.7 with 96).
 template <typename T, Mode MODE, Loss LOSS>
-int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
+int launch_type(const Args& given, int device, bool early, cudaStream_t stream) {
+    Args a = given;
     const int64_t bytes = a.rows.vocab * static_cast<int64_t>(sizeof(T)), grid = a.rows.batch * a.rows.length;
     // Fewer rows than multiprocessors: clusters of blocks split them, as long as a block has 8 KB to read.
     const int sms = tk_ops::sm_count(device);
     int shares = 1;
     while (shares < kMostShares && grid * shares * 2 <= sms && bytes / (shares * 2) >= 8 * 1024) shares *= 2;
-    if (shares > 1) return launch_clusters(token_rows_kernel<T, MODE, LOSS, 256, 2, true>, grid * shares, shares, 256, 0, early, stream, a, 0);
-    if (bytes <= 16 * 1024 && grid > 4 * sms) return launch(token_rows_kernel<T, MODE, LOSS, 96, 18, false>, grid, 96, 0, early, stream, a, 0);
+    if (shares > 1) {
+        a.first_rows = grid;
+        return launch_clusters(token_rows_kernel<T, MODE, LOSS, 256, 2, true>, grid * shares, shares, 256, 0, early, stream, a, 0);
+    }
+    // With `blocks` of them resident on a multiprocessor.
+    const auto rows = [&](auto kernel, int threads, int blocks, int kept) {
+        a.first_rows = static_cast<int64_t>(blocks) * sms;
+        return launch(kernel, grid, threads, static_cast<size_t>(kept) * 16, early, stream, a, kept);
+    };
+    if (bytes <= 16 * 1024 && grid > 4 * sms) return rows(token_rows_kernel<T, MODE, LOSS, 96, 18, false>, 96, 18, 0);
     if constexpr (MODE != kBoth) {
-        if (bytes > 16 * 1024) return launch(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, grid, 512, 0, early, stream, a, 0);
+        if (bytes > 16 * 1024) return rows(token_rows_kernel<T, MODE, LOSS, 512, 3, false>, 512, 3, 0);
     } else if (bytes > 80 * 1024 && a.in_phase) {
         auto kernel = token_rows_kernel<T, MODE, LOSS, 640, 2, false>;
         static std::atomic<bool> sized[64];
@@ -734,9 +744,9 @@ int launch_type(const Args& a, int device, bool early, cudaStream_t stream) {
             if (int code = check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptVectors * 16), "sizing shared memory")) return code;
             if (device < 64) sized[device].store(true, std::memory_order_relaxed);
         }
-        return launch(kernel, grid, 640, kKeptVectors * 16, early, stream, a, kKeptVectors);
+        return rows(kernel, 640, 2, kKeptVectors);
     }
-    return launch(token_rows_kernel<T, MODE, LOSS, 256, 6, false>, grid, 256, 0, early, stream, a, 0);
+    return rows(token_rows_kernel<T, MODE, LOSS, 256, 6, false>, 256, 6, 0);
 }
 
 template <Mode MODE, Loss LOSS>
