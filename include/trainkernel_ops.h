@@ -63,8 +63,10 @@ typedef struct {
     int32_t average;                                         /* TK_AVERAGE_* */
 } tk_policy_terms;
 
-/* Dense FP32 results of [batch, length] rows: `logprobs`, and, where not NULL, `stats` ([rows][2]: the row's largest
- * logit and the sum of exp(logit - largest)), which tk_token_logits_grad takes. */
+/* Dense FP32 results of [batch, length] rows: `logprobs`, and, where not NULL, `stats` ([rows][2]), which are made for
+ * tk_token_logits_grad and handed to it unchanged: the row's largest logit, and the sum of exp(logit - largest) times a
+ * factor between 2^-1/256 and 2^1/256 (1 where |largest| is 0 or above 65536) that depends on `largest` alone and that
+ * the gradient takes into account.  A log-sum-exp is the target's logit less its logprob, not largest + log(sum). */
 int tk_token_logprobs(const tk_token_rows* rows, float* logprobs, float* stats, int device, void* stream);
 
 /* logprobs and grad = scale * d(sum weights * logprobs)/d logits, each logit read from memory once where it fits. */

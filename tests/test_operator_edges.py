@@ -261,3 +261,20 @@ def test_policy_loss_of_many_rows_without_a_batch(rows, vocab, dtype, counted):
         assert torch.equal(got == 0, ~mask) and bool((grad[~mask] == 0).all()) and bool((grad[mask] != 0).any())
         assert abs(float(loss) - want) <= 2 * float(advantages.abs().max()) * (d + 8 * U) + 4 * U * abs(want)
         assert abs(float(tk.policy_loss(logits, targets, old, advantages, mask=mask, clip=(0.5, 1.0))[0]) - want) <= 2 * float(advantages.abs().max()) * (d + 8 * U) + 4 * U * abs(want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_saved_statistics_are_what_the_header_says(dtype):
+    """The sum is exact to rounding where the largest logit is 0 or beyond 2^16, elsewhere up to 2^(1/256) from it."""
+    from trainkernel_b200 import losses
+    tops = torch.tensor([0.0, 1.7, -3.3, 1000.1, -60000.7, 65535.9, 70000.0, -1e9, 1e30], device="cuda")
+    logits = (tops[:, None] + torch.zeros(9, 3001, device="cuda")).to(dtype)
+    logits[:, 1000:] = -float("inf")
+    targets = torch.full((9,), 5, dtype=torch.int64, device="cuda")
+    logp, stats = losses._logprobs_launch(logits, targets, None, True)
+    assert torch.equal(stats[:, 0], logits[:, 5].float())
+    ratio = (stats[:, 1].double() / 1000).log2().abs()
+    assert bool((ratio <= 1 / 256 + 16 * U).all())
+    assert bool((ratio[(logits[:, 5] == 0) | (logits[:, 5].float().abs() > 65536)] <= 16 * U).all())
+    assert bool(((logits[:, 5].double() - logp.double()) - (logits[:, 5].double() + math.log(1000)) <= 64 * U * logits[:, 5].double().abs().clamp(min=1)).all())
