@@ -277,4 +277,4 @@ def test_saved_statistics_are_what_the_header_says(dtype):
     ratio = (stats[:, 1].double() / 1000).log2().abs()
     assert bool((ratio <= 1 / 256 + 16 * U).all())
     assert bool((ratio[(logits[:, 5] == 0) | (logits[:, 5].float().abs() > 65536)] <= 16 * U).all())
-    assert bool(((logits[:, 5].double() - logp.double()) - (logits[:, 5].double() + math.log(1000)) <= 64 * U * logits[:, 5].double().abs().clamp(min=1)).all())
+    assert bool(((-logp.double() - math.log(1000)).abs() <= 64 * U).all())
