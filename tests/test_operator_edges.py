@@ -278,3 +278,40 @@ def test_saved_statistics_are_what_the_header_says(dtype):
     assert bool((ratio <= 1 / 256 + 16 * U).all())
     assert bool((ratio[(logits[:, 5] == 0) | (logits[:, 5].float().abs() > 65536)] <= 16 * U).all())
     assert bool(((-logp.double() - math.log(1000)).abs() <= 64 * U).all())
+
+
+# -- constants inside a transform ----------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("layout", ["dense", "shifted"])
+@pytest.mark.parametrize("long_way", [False, True])
+def test_constant_logits_inside_a_transform(layout, long_way, monkeypatch):
+    """The reference model's log-probabilities are computed inside the function that is differentiated, from logits that are not."""
+    from trainkernel_b200 import operators
+    logits, constant = noise((4, 6, 33), 1.0, 17)[:, :5], noise((4, 6, 33), 1.0, 18)[:, :5]
+    if layout == "dense":
+        logits, constant = logits.contiguous(), constant.contiguous()
+    targets = torch.randint(0, 33, (4, 5), generator=torch.Generator(device="cuda").manual_seed(19), device="cuda")
+    ref = tk.token_logprobs(constant, targets)
+    if long_way:
+        monkeypatch.setattr(operators, "fast", None)
+
+    def of_everything(x):
+        inside = tk.token_logprobs(constant, targets)
+        sums = tk.preference_loss(constant, targets, ref[:, 0])[1]
+        other, also, grad = tk.policy_loss_and_grad(constant, targets, inside, inside)
+        scored, weighed = tk.token_logprobs_and_grad(constant, targets, inside)
+        total = grad.float().sum() + weighed.float().sum() + tk.preference_loss_and_grad(constant, targets, sums)[0] + tk.policy_loss(constant, targets, also, scored)[0]
+        return tk.policy_loss(x, targets, inside, torch.ones_like(inside), ref_logprobs=inside, kl_weight=0.1)[0] + other + 0.0 * total
+
+    def directly(x):
+        return tk.policy_loss(x, targets, ref, torch.ones_like(ref), ref_logprobs=ref, kl_weight=0.1)[0] + tk.policy_loss(constant, targets, ref, ref)[0]
+
+    leaf = logits.clone().requires_grad_()
+    value = directly(leaf)
+    value.backward()
+    grad, got = torch.func.grad_and_value(of_everything)(logits)
+    torch.testing.assert_close(got, value.detach(), rtol=16 * U, atol=16 * U)
+    torch.testing.assert_close(grad, leaf.grad, rtol=16 * U, atol=1e-30)
+    torch.func.jvp(lambda y: y * tk.token_logprobs(constant, targets).sum(), (ref,), (ref,))
+    torch.testing.assert_close(torch.vmap(lambda y: y + tk.token_logprobs(constant, targets)[0, 0])(ref[0]), ref[0] + ref[0, 0])

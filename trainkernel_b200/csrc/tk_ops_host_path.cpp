@@ -32,7 +32,10 @@ bool plain(PyObject* object) {
     return !t._fw_grad(0).defined();                           // a tangent is refused there
 }
 
-bool tracing() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+// Inside a `torch.func` transform, too, what is allocated here would belong to it.
+bool tracing() {
+    return c10::impl::TorchDispatchModeTLS::any_modes_set() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
 
 bool number(PyObject* object, double* value) {
     if (PyFloat_CheckExact(object)) *value = PyFloat_AS_DOUBLE(object);

@@ -20,9 +20,11 @@ No counterpart in the reference, whose losses are means of squares (reference: b
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
+from torch._functorch.pyfunctorch import temporarily_clear_interpreter_stack
 from torch.autograd import forward_ad
 
 from . import operators
@@ -141,6 +143,18 @@ def _check_policy(who, logits, targets, old, advantages, ref, mask, clip, kl_wei
 # launches
 # ---------------------------------------------------------------------------
 
+def _outside_transforms(launch):
+    """A launch on plain tensors inside a `torch.func` transform of something else: its results are allocated as the
+    constants that they are, where the transform would wrap them."""
+    @functools.wraps(launch)
+    def run(*args, **kwargs):
+        if torch._C._functorch.peek_interpreter_stack() is None:
+            return launch(*args, **kwargs)
+        with temporarily_clear_interpreter_stack():
+            return launch(*args, **kwargs)
+    return run
+
+
 def _array(value: torch.Tensor | None, rank: int) -> tuple:
     """(pointer, batch stride, token stride) of a [batch, length] or [rows] tensor."""
     if value is None:
@@ -197,6 +211,7 @@ def _grad_struct(grad: torch.Tensor | None, scale: float, scale_at: torch.Tensor
     return TokenGrad(grad.data_ptr(), strides[0] if grad.dim() == 3 else 0, strides[-2], _pointer(scale_at), scale, 0)
 
 
+@_outside_transforms
 def _logprobs_launch(logits, targets, mask, with_stats: bool):
     lib, device, stream = _place(logits)
     logprobs = _fp32(targets.shape, logits)
@@ -205,6 +220,7 @@ def _logprobs_launch(logits, targets, mask, with_stats: bool):
     return logprobs, stats
 
 
+@_outside_transforms
 def _logprobs_and_grad_launch(logits, targets, weights, mask, scale: float, scale_at):
     lib, device, stream = _place(logits)
     logprobs = _fp32(targets.shape, logits)
@@ -214,6 +230,7 @@ def _logprobs_and_grad_launch(logits, targets, weights, mask, scale: float, scal
     return logprobs, grad
 
 
+@_outside_transforms
 def _logits_grad_launch(logits, targets, mask, coefficients, stats, scale_at):
     lib, device, stream = _place(logits)
     grad = _grad_like(logits)
@@ -226,6 +243,7 @@ def _logits_grad_launch(logits, targets, mask, coefficients, stats, scale_at):
     return grad
 
 
+@_outside_transforms
 def _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_weight, average: int, *, saved: bool, grad: bool,
                    scale: float = 1.0, scale_at=None):
     lib, device, stream = _place(logits)
@@ -242,6 +260,7 @@ def _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_we
     return loss, logprobs, stats, coefficients, out
 
 
+@_outside_transforms
 def _preference_launch(logits, targets, reference, mask, beta: float, smoothing: float, *, grad: bool, scale: float = 1.0, scale_at=None):
     lib, device, stream = _place(logits)
     shape = targets.shape
@@ -484,7 +503,7 @@ def token_logprobs_and_grad(logits: torch.Tensor, targets: torch.Tensor, weights
     _check_rows(who, logits, targets, mask)
     weights = _check_constant(who, "weights", weights, targets.shape, logits.device)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits, targets, weights, mask):
+    if _is_plain(logits, targets, weights, mask, scale_at):
         return _logprobs_and_grad_launch(logits, targets, weights, mask, scale, scale_at)
     _no_tensor_scale(who, scale_at)
     return _call.token_logprobs_and_grad(logits, targets, weights, mask, scale)
@@ -522,7 +541,7 @@ def policy_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, old_logpro
     who = "policy_loss_and_grad"
     old, advantages, ref, low, high, kl_weight, which = _check_policy(who, logits, targets, old_logprobs, advantages, ref_logprobs, mask, clip, kl_weight, average)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits, targets, old, advantages, ref, mask):
+    if _is_plain(logits, targets, old, advantages, ref, mask, scale_at):
         loss, logprobs, _, _, grad = _policy_launch(logits, targets, old, advantages, ref, mask, low, high, kl_weight, which, saved=False, grad=True,
                                                     scale=scale, scale_at=scale_at)
         return loss, logprobs, grad
@@ -567,7 +586,7 @@ def preference_loss_and_grad(logits: torch.Tensor, targets: torch.Tensor, refere
     who = "preference_loss_and_grad"
     reference, beta, label_smoothing = _check_preference(who, logits, targets, reference, mask, beta, label_smoothing)
     scale, scale_at = _check_scale(who, grad_scale, logits.device)
-    if _is_plain(logits, targets, reference, mask):
+    if _is_plain(logits, targets, reference, mask, scale_at):
         loss, sums, _, _, grad = _preference_launch(logits, targets, reference, mask, beta, label_smoothing, grad=True, scale=scale, scale_at=scale_at)
         return loss, sums, grad
     _no_tensor_scale(who, scale_at)
