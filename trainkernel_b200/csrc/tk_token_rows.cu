@@ -63,6 +63,7 @@ template <typename T> struct Vector;
 template <> struct Vector<float> {
     static constexpr int kCount = 4;
     static constexpr bool kSplit = false;          // whether gradients need exp2_split
+    static constexpr bool kWide = true;            // whether finite logits reach beyond kExtreme
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[2]) {
         f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
         f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
@@ -79,6 +80,7 @@ template <> struct Vector<float> {
 template <> struct Vector<__nv_bfloat16> {
     static constexpr int kCount = 8;
     static constexpr bool kSplit = false;
+    static constexpr bool kWide = true;
     static __device__ __forceinline__ float2 two(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
         f[0] = two(v.x);
@@ -102,6 +104,7 @@ template <> struct Vector<__nv_bfloat16> {
 template <> struct Vector<__half> {
     static constexpr int kCount = 8;
     static constexpr bool kSplit = true;
+    static constexpr bool kWide = false;
     static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[4]) {
         const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
@@ -152,11 +155,8 @@ __device__ __forceinline__ float shift(float from, const Exponent& to) {
     return far ? fmaf(from, kLog2e, -to.base) : scaled(from) - to.base;
 }
 
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float top = fmaxf(a.top, b.top);
-    const Exponent e(top);
-    return {top, a.sum * exp2_fast(shift(a.top, e)) + b.sum * exp2_fast(shift(b.top, e))};
-}
+// The same statistics relative to a top that is as large or larger.
+__device__ __forceinline__ Stat raised(Stat s, float top) { return {top, s.sum * exp2_fast(shift(s.top, Exponent(top)))}; }
 
 // 2^(x log2(e) - base) with the exponent split at a whole number, so that its fraction keeps all of its bits: the rounding of
 // an exponent near -12 alone costs 2^-21 of the value, more than one part in a hundred of half a step of FP16, and with small
@@ -175,8 +175,10 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, Vector<T>::top(v[i]));
     const Exponent e(top);
-    if (!e.extreme) {
-        s.sum *= exp2_fast(shift(s.top, e));               // 0 while nothing was added
+    // Both tops within kExtreme, or nothing added yet (or only what is nothing beside the new top): the short form of `raised`.
+    const bool far = e.extreme || (Vector<T>::kWide && s.top < -kExtreme && s.top != kLowest);
+    if (!far) {
+        s.sum *= exp2_fast(scaled(s.top) - e.base);
         s.top = top;
         const Pair scale = pair(kLog2e, kLog2e), base = pair(-e.base, -e.base);
         Pair sum = pair(0.f, 0.f);
@@ -193,7 +195,7 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
         const float2 total = both(sum);
         s.sum += total.x + total.y;
     } else {
-        s = join(s, {top, 0.f});
+        s = raised(s, top);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float2 f[kPairs];
@@ -207,7 +209,7 @@ __device__ __forceinline__ void accumulate(Stat& s, const uint4 (&v)[N]) {
 template <typename T>
 __device__ __forceinline__ void accumulate_one(Stat& s, T value) {
     const float x = Vector<T>::load(value);
-    if (x > s.top) s = join(s, {x, 0.f});
+    if (x > s.top) s = raised(s, x);
     s.sum += exp2_fast(Exponent(s.top)(x));
 }
 
@@ -251,7 +253,7 @@ __device__ __forceinline__ Stat warp_join(Stat mine) {
     float top = mine.top;
 #pragma unroll
     for (int step = 16; step; step >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, step));
-    float sum = join(mine, {top, 0.f}).sum;
+    float sum = raised(mine, top).sum;
 #pragma unroll
     for (int step = 16; step; step >>= 1) sum += __shfl_xor_sync(~0u, sum, step);
     return {top, sum};
