@@ -324,8 +324,9 @@ __device__ __forceinline__ unsigned long long keep_policy() {
 constexpr int kAhead = 4;                      // vectors a thread has in flight
 
 // Asks L2 for the vectors of a thread's next turn before it loads those of this one: registers for a second set in flight
-// would cost resident blocks.  8000 x 32000 BF16 logits with gradient: 198 -> 179 us; two or three turns ahead 186 and 190.
-// The statistics alone, whose blocks only read, are a little faster without (8192 x 128256: 353 us against 360).
+// would cost resident blocks.  Policy loss of 8000 x 32000 BF16 logits with gradient, in the block shape it had then: 198 ->
+// 179 us; two or three turns ahead 186 and 190.  The statistics alone, whose blocks only read, do without: asking ahead
+// takes 113 us instead of 110 at that size and 338 instead of 349 at 8192 x 128256.
 template <int THREADS>
 __device__ __forceinline__ void prefetch_turn(const uint4* body, int i, int end) {
     if (threadIdx.x % 8) return;                           // one request for every 128 bytes
@@ -490,7 +491,7 @@ __device__ __forceinline__ Stat cluster_join(Stat mine, const Share share, float
 
 // One block per row, or, with SPLIT, one cluster of blocks per row.  Memory bounds the statistics alone; with the gradient a
 // block waits for its join between the passes, which only the other blocks of the multiprocessor fill, and every logit
-// takes two exponentials (65 % of their unit at 8000 x 32000 BF16).  launch_type has the block shapes and their times.
+// takes two exponentials (72 % of their unit's cycles at 4000 x 32000 BF16, 63 % at 1024 x 128256).  launch_type has the block shapes and their times.
 template <typename T, Mode MODE, Loss LOSS, int THREADS, int BLOCKS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, BLOCKS) token_rows_kernel(const __grid_constant__ Args a, const int kept) {
     extern __shared__ uint4 kept_at[];
@@ -712,13 +713,15 @@ int launch(void (*kernel)(A...), int64_t grid, int threads, size_t shared, bool 
 constexpr int kKeptVectors = 2 * kAhead * 640;             // 80 KB
 
 // How many threads share a row, and so how many rows are in flight.  More, smaller blocks hide one another's joins until
-// registers run out: 16384 x 8000 BF16 logits with gradient take 106 us with 18 blocks of 96 threads on an SM, 111 with 24 of
-// 64, 116 with 16 of 128, 149 with 8 of 256; rows of 62 KB (8000 of them) take 176 us with 6 blocks of 256 threads, 179 with
-// 5, 185 with 4, 194 with 8 of 192, 196 with 3 of 512.  For long rows the second read has to find the row in L2, so few rows
-// may be in flight: 4096 rows of 250 KB take 363 us with 2 blocks of 640 threads that keep the first 80 KB of their row in
-// shared memory; before L2 was asked ahead 394, 417 without keeping, 444 with 3 blocks of 512.  The statistics alone take
-// 158 us of those rows with 3 blocks of 512 threads, 161 with 6 of 256, 176 with 8 of 256.  Short rows that all run at once
-// get more threads each (256 x 1000 FP32 with gradient, captured: 7.0 us with 256, 7.2 with 128, 8.7 with 96).
+// registers run out: a policy loss of 16384 x 8000 BF16 logits with gradient takes 104 us with 18 blocks of 96 threads on an
+// SM, 115 with 24 of 64, 120 with 16 of 128, 151 with 8 of 256; 8000 rows of 62 KB take 174 us with 6 blocks of 256 threads,
+// 178 with 5, 183 with 4, 190 with 8 of 192, 199 with 3 of 512.  (The form with given weights holds more across its loops
+// and spills in these shapes: 110 and 189 us.)  For long rows the second read has to find the row in L2, so few rows may be
+// in flight: 4096 rows of 250 KB take 366 us with 2 blocks of 640 threads that keep the first 80 KB of their row in shared
+// memory; before L2 was asked ahead 394, 417 without keeping, 444 with 3 blocks of 512.  The statistics alone take 110 us of
+// 8000 x 32000 and 349 of 8192 x 128256 BF16 logits with 3 blocks of 512 threads; 6 of 256 take 89 and 323, 8 of 256 88 and 314.
+// Short rows that all run at once get more threads each (256 x 1000 FP32 with gradient, captured: 6.7 us with 256 threads;
+// when it was 7.0, 7.2 with 128 and 8.7 with 96).
 template <typename T, Mode MODE, Loss LOSS>
 int launch_type(const Args& given, int device, bool early, cudaStream_t stream) {
     Args a = given;

@@ -15,7 +15,7 @@ strides as long as one row is contiguous, so the usual shifted slice `logits[:, 
 `targets` are int64 or int32.  `mask` is boolean, of the targets' shape; a row it excludes has
 log-probability 0 and gradient 0 whatever its logits hold, NaN included.  A counted target outside
 `[0, vocab)` reads nothing and gives NaN.  Log-probabilities, losses and sums are FP32; gradients have
-the logits' type, and, for strided logits, their strides.  Everything else that enters a loss is a constant: it must not require grad.
+the logits' type, and, for strided logits, their strides (inside a traced or transformed function they are dense).  Everything else that enters a loss is a constant: it must not require grad.
 No counterpart in the reference, whose losses are means of squares (reference: benchmarks/train_loop.py:35-45).
 """
 from __future__ import annotations
@@ -512,7 +512,8 @@ def token_logprobs_and_grad(logits: torch.Tensor, targets: torch.Tensor, weights
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
                 ref_logprobs: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip: tuple[float, float] = (0.2, 0.2),
                 kl_weight: float = 0.0, average: str = "tokens") -> tuple[torch.Tensor, torch.Tensor]:
-    """`(loss, logprobs)` of the clipped policy objective with a KL penalty; the loss is differentiable in the logits.
+    """`(loss, logprobs)` of the clipped policy objective with a KL penalty; the loss is differentiable in the logits,
+    `logprobs` is a constant beside it.
 
     Per counted token, with `r = exp(logprob - old_logprob)`:
     `-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_weight (exp(d) - d - 1)`, `d = ref_logprob - logprob`.
@@ -559,7 +560,7 @@ def _check_preference(who, logits, targets, reference, mask, beta, label_smoothi
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: torch.Tensor, *, mask: torch.Tensor | None = None,
                     beta: float = 0.1, label_smoothing: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
-    """`(loss, sums)` over pairs of sequences; the loss is differentiable in the logits.
+    """`(loss, sums)` over pairs of sequences; the loss is differentiable in the logits, `sums` is a constant beside it.
 
     Sequence `i` is preferred over sequence `i + batch / 2`.  `sums[i]` is the sum of sequence i's counted
     log-probabilities, `reference[i]` the same sum under the reference model; with
