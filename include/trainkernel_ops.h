@@ -121,8 +121,9 @@ typedef struct {
 } tk_adamw_options;
 
 /* All tensors share the parameter type and the gradient type.  No parameter overlaps another one, the state, a gradient
- * other than its own (which may be the same memory, element for element) or the values at lr_at and scale_at.  `last`: non-zero on the last call of one optimizer
- * step (a step over tensors of several types takes several calls): that call advances the step counters. */
+ * other than its own (which may be the same memory, element for element) or the values at lr_at and scale_at.
+ * `last`: non-zero on the last call of one optimizer step (a step over tensors of several types takes several calls):
+ * that call advances the step counters. */
 int tk_adamw_update(const tk_adamw_tensor* tensors, int count, int param_dtype, int grad_dtype, const tk_adamw_state* state,
                     const tk_adamw_options* options, int last, int device, void* stream);
 

@@ -53,6 +53,20 @@ def test_a_saved_state_of_another_order_is_refused():
         target.load_state_dict({key: value for key, value in saved.items() if key != "paths"})       # saved without names
 
 
+def test_containers_without_keys_go_by_position():
+    from torch.utils import _pytree
+
+    class Pair:
+        def __init__(self, a, b):
+            self.a, self.b = a, b
+
+    _pytree.register_pytree_node(Pair, lambda pair: ([pair.a, pair.b], None), lambda children, _: Pair(*children))
+    tree = {"layer": Pair(torch.zeros(3), torch.zeros(4))}
+    for params in (tree, [torch.zeros(3), torch.zeros(4)]):
+        with pytest.raises(RuntimeError, match="sm_100a GPU required"):
+            tk.AdamW().update(params, tree, state_of(tree))
+
+
 @gpu
 def test_a_tree_is_updated_by_its_names():
     optimizer, params = tk.AdamW(lr=0.1, weight_decay=0.0), tree_of("qkv", "cuda")

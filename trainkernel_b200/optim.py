@@ -112,10 +112,14 @@ def _leaves(tree: Any, what: str) -> list[torch.Tensor]:
 
 
 def _paths(tree: Any) -> tuple[str, ...] | None:
-    """Where every tensor of a tree stands; None for a tensor or a plain list or tuple of them, which go by position alone."""
+    """Where every tensor of a tree stands; None for a tensor, for a plain list or tuple of them and for containers registered
+    without keys, which go by position alone."""
     if isinstance(tree, torch.Tensor) or isinstance(tree, (list, tuple)) and all(isinstance(x, torch.Tensor) for x in tree):
         return None
-    return tuple(keystr(path) for path, _ in tree_flatten_with_path(tree)[0])
+    try:
+        return tuple(keystr(path) for path, _ in tree_flatten_with_path(tree)[0])
+    except ValueError:
+        return None
 
 
 def _names(paths: Any) -> tuple[str, ...] | None:
@@ -252,9 +256,10 @@ class AdamW:
         """One step, in place, on the current stream.
 
         `params` and `grads` are trees of the structure that `init` was given, or plain lists in the order of its leaves.
-        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16).  No two params overlap in memory, and nothing else
-        overlaps one, but a gradient its own param.  `grad_scale` (one FP32 value on the device, for clipping or for undoing a loss scale) multiplies the gradients; when it is not finite the step does
-        not happen: parameters, moments and step count stay as they are.
+        `grads` matches `params` in shape and memory order (FP32, FP16 or BF16).  No two params overlap in memory, and
+        nothing else overlaps one, but a gradient its own param.  `grad_scale` (one FP32 value on the device, for clipping
+        or for undoing a loss scale) multiplies the gradients; when it is not finite the step does not happen: parameters,
+        moments and step count stay as they are.
         """
         if operators.fast is not None and state.bits == self.state_bits and operators.fast.adamw_update(
                 params, grads, state.sizes, state.offsets, self.weight_decay, state._struct_at, state._tensors, self.state_bits, self.lr, self.betas,
